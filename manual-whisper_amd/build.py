@@ -18,7 +18,10 @@ LIB = os.path.join(HERE, "libmwhip.so")
 SOURCES = ["engine.hip", "kernels_mel.hip", "kernels_gemm.hip", "kernels_enc.hip", "kernels_dec.hip", "kernels_vad.hip", "kernels_w2v.hip", "aligner.hip"]
 HEADERS = [os.path.join(CSRC, "mw_kernels.h"), os.path.join(os.path.dirname(HERE), "include", "mwhip.h")]
 ARCH = "gfx950"
-FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-function"]
+# no packed fp32 instructions: some forms of v_pk_add/mul/fma_f32, which the compiler makes of ordinary float code, have
+# given wrong results on these GPUs now and then
+ARCH_FLAGS = [f"--offload-arch={ARCH}", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+FLAGS = ["-O3", "-std=c++17", "-fPIC"] + ARCH_FLAGS + ["-Wall", "-Wno-unused-function"]
 # kernels_enc.hip: the encoder attention takes maxima of MFMA results; told that no NaN needs quieting, the compiler
 # drops a `v_max x, x` per operand (44 of the 58 max instructions of a key tile)
 EXTRA_FLAGS = {"kernels_enc.hip": ["-fno-honor-nans"]}
@@ -82,7 +85,7 @@ def build_gemm_check(force: bool = False, verbose: bool = True) -> str:
     if force or _stale(exe, [src, obj] + HEADERS):
         hipcc = _hipcc()
         tmp = os.path.join(root, "tools", "gemm_bench.o")
-        for cmd in ([hipcc, "-O3", "-std=c++17", f"--offload-arch={ARCH}", "-I", CSRC, "-c", src, "-o", tmp],
+        for cmd in ([hipcc, "-O3", "-std=c++17"] + ARCH_FLAGS + ["-I", CSRC, "-c", src, "-o", tmp],
                     [hipcc, f"--offload-arch={ARCH}", tmp, obj, "-o", exe]):
             if verbose:
                 print(" ".join(cmd), flush=True)
@@ -101,7 +104,7 @@ def build_attention_check(force: bool = False, verbose: bool = True) -> str:
     if force or _stale(exe, [src, obj] + HEADERS):
         hipcc = _hipcc()
         tmp = os.path.join(root, "tools", "attn_bench.o")
-        for cmd in ([hipcc, "-O3", "-std=c++17", f"--offload-arch={ARCH}", "-I", CSRC, "-c", src, "-o", tmp],
+        for cmd in ([hipcc, "-O3", "-std=c++17"] + ARCH_FLAGS + ["-I", CSRC, "-c", src, "-o", tmp],
                     [hipcc, f"--offload-arch={ARCH}", tmp, obj, "-o", exe]):
             if verbose:
                 print(" ".join(cmd), flush=True)
