@@ -43,7 +43,7 @@ typedef enum {
     MW_ERR_NOMEM = -6
 } mw_status;
 
-typedef enum { MW_F32 = 0, MW_F16 = 1, MW_BF16 = 2 } mw_dtype;
+typedef enum { MW_F32 = 0, MW_F16 = 1, MW_BF16 = 2, MW_E4M3 = 3 /* caches in pages only */ } mw_dtype;
 
 /* How the engine keeps the Linear weights of the encoder and decoder layers in HBM (what the
  * compute_type argument of whisperx.load_model, reference transcribe.py:32,109, selects there).
@@ -130,7 +130,8 @@ int mw_fork_cached(mw_ctx* parent, int max_batch, int cache_sequences, mw_ctx** 
 /* Free everything the context owns (reference transcribe.py:153-154 `del model`). */
 void mw_destroy(mw_ctx* ctx);
 
-/* Message of the most recent failure on this context (or of mw_create when ctx is NULL). */
+/* Message of the most recent failure on this context (ctx NULL: of mw_create, or of a call that takes no context, on this
+ * thread). */
 const char* mw_last_error(const mw_ctx* ctx);
 
 /* ---- the hot path: model.transcribe (reference transcribe.py:123) ---- */
@@ -284,6 +285,139 @@ int mw_profile_decode_gemvs(mw_ctx* ctx, int batch, int iters, float* mean_ms_pe
 int mw_set_option(mw_ctx* ctx, const char* key, int value);
 
 int mw_synchronize(mw_ctx* ctx);
+
+/* ------------------------------------------------------------------------------------------------
+ * Drafted tokens over a K/V cache in pages: the operators of one step of drafted (speculative) decoding.  No counterpart in
+ * the reference's call surface, whose backend decodes token by token behind model.transcribe (reference transcribe.py:123).
+ *
+ * A cache holds pages of page_size tokens; the pages of request b, in order, are table[b][0..].  Request b has kept[b]
+ * tokens in its pages and appends fresh[b] rows in a step: the nodes of a tree of drafted tokens, every parent before its
+ * children, node 0 the root (a token that is certain, whose K/V are not cached yet), or without parents a chain.  Row
+ * row_start[b] + i is node i; its K/V go to cache position kept[b] + i whatever its depth.  A step is
+ *     mw_paged_plan -> per layer: mw_paged_write, mw_tree_attention -> mw_tree_accept -> mw_paged_compact
+ * after which kept[b] grows by count[b], and the next plan takes back the pages that are no longer needed.
+ *
+ * These calls differ from those that take a context: every array is device memory of GPU `device` (4-byte integers unless
+ * said otherwise), nothing is allocated, the launches are queued on `stream` (a hipStream_t of that GPU; NULL: its default
+ * stream) and the call returns at once; it can be captured into a graph.  The calls are stateless and may run on any number
+ * of threads and streams; two calls that may overlap need workspaces of their own.  A bad argument is refused before
+ * anything is queued; what only the device can see (page ids, slots, parents, lengths) is checked there: an index outside
+ * its buffer is never used, and what follows then is said at each call.  The calling thread's current device is left as
+ * it was.
+ * ------------------------------------------------------------------------------------------------ */
+
+/* One layer of a cache: row (page, head, offset) of K starts page * page_stride + head * head_stride + offset * token_stride
+ * elements behind k (V: behind v), head_dim values side by side; strides and bases are multiples of 16 bytes.
+ * dtype MW_F16, MW_BF16, or MW_E4M3: OCP codes with one fp32 scale per row (max|.| / 448, round to nearest even) in
+ * k_scale / v_scale [n_pages][n_heads][page_size]. */
+typedef struct {
+    void* k; void* v;
+    float* k_scale; float* v_scale;       /* MW_E4M3 only, else NULL      */
+    int64_t page_stride, head_stride, token_stride;
+    int32_t n_pages;                      /* n_pages * page_size < 2^31   */
+    int32_t page_size;                    /* a power of two in 16..4096   */
+    int32_t n_heads;                      /* K/V heads                    */
+    int32_t head_dim;                     /* 64 or 128                    */
+    int32_t dtype;
+} mw_paged_cache;
+
+typedef struct {
+    int32_t batch;                        /* requests, 1..2048                                                          */
+    int32_t rows;                         /* capacity of the row arrays; the rows of a step are sum(fresh)               */
+    int32_t page_size, n_pages;
+    int32_t max_pages;                    /* entries of a table row that may be used                                    */
+    const int32_t* kept;                  /* [batch]                                                                    */
+    const int32_t* fresh;                 /* [batch]                                                                    */
+    const int32_t* parents;               /* [rows] index within the tree, -1 = none; NULL: chains                      */
+    int32_t* table; int64_t table_stride; /* [batch][table_stride], updated in place                                    */
+    const int32_t* pages_in; int32_t* pages_out;     /* [batch] pages each request holds, before and after              */
+    int32_t* free_list;                   /* [n_pages] stack of free pages, updated in place                            */
+    const int32_t* n_free_in; int32_t* n_free_out;   /* [1] entries on the stack, before and after                      */
+    int32_t* row_start;                   /* [batch + 1] out                                                            */
+    int32_t* admitted;                    /* [batch] out: 1 = the request has its pages                                 */
+    int64_t* slots;                       /* [rows] out: page * page_size + offset, or -1                               */
+    int32_t* positions;                   /* [rows] out: kept + depth in the tree (chains: + index), or -1              */
+    uint32_t* mask; int32_t mask_words;   /* [rows][mask_words] out, with parents: bit j = node j is an ancestor or the
+                                           * node itself; at most 32 * mask_words nodes a tree, 1..8 words              */
+    int32_t* units; int32_t* unit_start;  /* optional out: [batch + chunk_units][4] (request, first key, key behind the
+                                           * last, units of that request; -1 behind the last unit) and [batch + 1]       */
+    int32_t chunk_units;                  /* pieces wanted in all: requests are cut into equal pieces of multiples of 64
+                                           * keys, none shorter than chunk_min; 0: no request is cut                    */
+    int32_t chunk_min;
+} mw_plan_args;
+
+/* The plan of a step from the lengths alone: pages, tables, slots, positions, tree masks and the work units of the
+ * attention.  Request b needs ceil((kept + fresh) / page_size) pages.  Pages it holds beyond that go back on the stack
+ * (in request order); pages it lacks are taken from the top of the stack as those returns leave it, request by request.
+ * A request is refused (admitted 0, slots -1, pages as they were) when the stack has not enough for it and the growing
+ * requests before it, when it would exceed max_pages, the rows' capacity or (trees) the mask, or when a length is negative;
+ * requests that need no new page are admitted whatever the stack holds.  A request without its lengths in range has
+ * positions -1 and an empty mask.  Rows behind the last request have slot -1, position -1 and an empty mask.  A parent that
+ * is not an earlier node of the same tree counts as none.  kept = fresh = 0 gives everything back.
+ * The step takes effect with pages_out / n_free_out: planning again from the same counts gives the same plan. */
+int mw_paged_plan(const mw_plan_args* args, int device, void* stream);
+
+/* K/V rows into their slots (-1, or beyond the cache: the row is dropped).  k, v [rows][cache heads][head_dim] of `dtype`
+ * MW_F16 or MW_BF16 with their strides in elements (views into fused q|k|v rows, say; multiples of 8); a 16-bit cache takes
+ * rows of its own type.  e4m3: a row that holds an infinity or a NaN reads back as NaN throughout.  No two rows may have
+ * the same slot. */
+int mw_paged_write(const mw_paged_cache* cache, const void* k, const void* v, int dtype, int64_t k_row_stride, int64_t k_head_stride,
+                   int64_t v_row_stride, int64_t v_head_stride, const int64_t* slots, int64_t rows, int device, void* stream);
+
+typedef struct {
+    mw_paged_cache cache;
+    const void* q; int64_t q_row_stride, q_head_stride;         /* [rows][n_heads][head_dim] of `dtype`                   */
+    void* out; int64_t out_row_stride, out_head_stride;         /* likewise                                              */
+    int32_t dtype;                        /* MW_F16 or MW_BF16; a 16-bit cache has the same type                        */
+    int32_t n_heads;                      /* query heads: a multiple of the cache's; head h reads K/V head h / (n_heads / cache heads) */
+    int32_t rows, batch;
+    int32_t max_nodes;                    /* no request has more rows (more are not computed)                           */
+    const int32_t* table; int64_t table_stride; int32_t max_pages;
+    const int32_t* kept; const int32_t* row_start;
+    const int32_t* units; const int32_t* unit_start; int32_t n_units;       /* of mw_paged_plan; n_units = batch + chunk_units */
+    const uint32_t* mask; int32_t mask_words;                   /* NULL: chains (node i sees nodes 0..i)                 */
+    float scale;                          /* of the scores, usually 1 / sqrt(head_dim)                                  */
+    void* workspace; int64_t workspace_bytes;       /* mw_tree_attention_workspace() bytes, 16-byte aligned              */
+} mw_tree_args;
+
+/* out[r][h] = sum_j p_j V[j], p = softmax over the keys j that row r sees of scale * q[r][h] . K[j]: all kept tokens of its
+ * request, and of the step's nodes those in its mask (bits may name any node of the request).  A row that sees nothing is
+ * zero, as are the rows of a request that was refused; rows behind the last request are left as they are.  Keys in a page
+ * that does not exist (id outside 0..n_pages-1) count as not seen.  What a row does not see never reaches it, infinities
+ * and NaN included.  Scores, maxima, sums and the result are held in fp32; weights are rounded once to `dtype` for the
+ * product with V.  mw_tree_attention_workspace returns bytes (0: no workspace) or a negative mw_status; it reads neither
+ * arrays nor workspace. */
+int64_t mw_tree_attention_workspace(const mw_tree_args* args);
+int mw_tree_attention(const mw_tree_args* args, int device, void* stream);
+
+typedef struct {
+    const void* logits; int64_t logits_stride;      /* [rows][vocab] of `dtype`: MW_F32, MW_F16 or MW_BF16               */
+    int32_t dtype, rows, vocab, batch;
+    int32_t depth;                        /* columns of path and out_tokens, 1..1024; nodes from `depth` on are not followed */
+    const uint8_t* suppress;              /* [vocab] or NULL: ids with a value other than 0 are never chosen            */
+    const int32_t* tokens;                /* [rows] the drafted tokens                                                  */
+    const int32_t* parents;               /* [rows]                                                                     */
+    const int32_t* row_start;             /* [batch + 1]                                                                */
+    int32_t* best;                        /* [rows] out: arg-max of every row that belongs to a request                 */
+    int32_t* path;                        /* [batch][depth] out: accepted nodes, -1 behind them                         */
+    int32_t* count;                       /* [batch] out: accepted nodes (0: the request has no rows)                   */
+    int32_t* out_tokens;                  /* [batch][depth] out: best[path], the tokens that follow                     */
+    void* workspace; int64_t workspace_bytes;       /* mw_tree_accept_workspace() bytes                                  */
+} mw_accept_args;
+
+/* Greedy acceptance: best[r] is the lowest id with the largest logit among those not suppressed (a NaN is never chosen; 0
+ * where nothing can be).  From node 0, which is always accepted, the path goes on to the lowest child whose token is the
+ * arg-max of the node it stands on. */
+int64_t mw_tree_accept_workspace(const mw_accept_args* args);
+int mw_tree_accept(const mw_accept_args* args, int device, void* stream);
+
+/* Accepted rows side by side: the K/V row at position kept[b] + path[b][i] moves to kept[b] + i for i < count[b], in all
+ * n_layers layers (layer l of K starts l * layer_stride elements behind cache->k, V likewise, and the scales follow each
+ * other layer by layer).  path [batch][path_stride] ascends; an entry smaller than its index is skipped, as is one whose
+ * page does not exist. */
+int mw_paged_compact(const mw_paged_cache* cache, int32_t n_layers, int64_t layer_stride, const int32_t* table, int64_t table_stride,
+                     int32_t max_pages, const int32_t* kept, const int32_t* path, int32_t path_stride, const int32_t* count,
+                     int32_t batch, int device, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Forced alignment: the acoustic model behind whisperx.load_align_model / whisperx.align

@@ -18,6 +18,8 @@ SYMBOLS = (
     "mw_frame_energy_db", "mw_stage_ms", "mw_profile_cross_attention", "mw_profile_decode_gemvs", "mw_set_option", "mw_synchronize",
     "mw_align_frames", "mw_align_create", "mw_align_destroy", "mw_align_last_error", "mw_align_set_weight", "mw_align_finalize",
     "mw_align_emissions", "mw_align_fork", "mw_align_path", "mw_align_segment", "mw_align_segments",
+    "mw_paged_plan", "mw_paged_write", "mw_tree_attention_workspace", "mw_tree_attention", "mw_tree_accept_workspace", "mw_tree_accept",
+    "mw_paged_compact",
 )
 
 
@@ -41,6 +43,37 @@ class AlignDesc(C.Structure):
     _fields_ = [("n_conv", C.c_int32), ("conv_dim", C.c_int32), ("conv_kernel", C.c_int32 * 8), ("conv_stride", C.c_int32 * 8),
                 ("hidden", C.c_int32), ("n_heads", C.c_int32), ("n_layers", C.c_int32), ("ffn_dim", C.c_int32),
                 ("pos_kernel", C.c_int32), ("pos_groups", C.c_int32), ("vocab", C.c_int32), ("max_samples", C.c_int32)]
+
+
+class PagedCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("token_stride", C.c_int64),
+                ("n_pages", C.c_int32), ("page_size", C.c_int32), ("n_heads", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32)]
+
+
+class PlanArgs(C.Structure):
+    _fields_ = [("batch", C.c_int32), ("rows", C.c_int32), ("page_size", C.c_int32), ("n_pages", C.c_int32), ("max_pages", C.c_int32),
+                ("kept", C.c_void_p), ("fresh", C.c_void_p), ("parents", C.c_void_p), ("table", C.c_void_p), ("table_stride", C.c_int64),
+                ("pages_in", C.c_void_p), ("pages_out", C.c_void_p), ("free_list", C.c_void_p), ("n_free_in", C.c_void_p),
+                ("n_free_out", C.c_void_p), ("row_start", C.c_void_p), ("admitted", C.c_void_p), ("slots", C.c_void_p),
+                ("positions", C.c_void_p), ("mask", C.c_void_p), ("mask_words", C.c_int32), ("units", C.c_void_p),
+                ("unit_start", C.c_void_p), ("chunk_units", C.c_int32), ("chunk_min", C.c_int32)]
+
+
+class TreeArgs(C.Structure):
+    _fields_ = [("cache", PagedCache), ("q", C.c_void_p), ("q_row_stride", C.c_int64), ("q_head_stride", C.c_int64),
+                ("out", C.c_void_p), ("out_row_stride", C.c_int64), ("out_head_stride", C.c_int64), ("dtype", C.c_int32),
+                ("n_heads", C.c_int32), ("rows", C.c_int32), ("batch", C.c_int32), ("max_nodes", C.c_int32), ("table", C.c_void_p),
+                ("table_stride", C.c_int64), ("max_pages", C.c_int32), ("kept", C.c_void_p), ("row_start", C.c_void_p),
+                ("units", C.c_void_p), ("unit_start", C.c_void_p), ("n_units", C.c_int32), ("mask", C.c_void_p),
+                ("mask_words", C.c_int32), ("scale", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
+class AcceptArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("logits_stride", C.c_int64), ("dtype", C.c_int32), ("rows", C.c_int32), ("vocab", C.c_int32),
+                ("batch", C.c_int32), ("depth", C.c_int32), ("suppress", C.c_void_p), ("tokens", C.c_void_p), ("parents", C.c_void_p),
+                ("row_start", C.c_void_p), ("best", C.c_void_p), ("path", C.c_void_p), ("count", C.c_void_p), ("out_tokens", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
 
 
 _lib = None
@@ -180,7 +213,18 @@ def load() -> C.CDLL:
     lib.mw_align_segment.argtypes = [vp, f32p, C.c_int64, vp, C.c_int32, C.c_int32, vp, vp, C.POINTER(C.c_int32)]
     lib.mw_align_segments.argtypes = [vp, C.c_int32, vp, vp, vp, vp, C.c_int32, vp, vp, vp, vp]
     lib.mw_align_path.argtypes = [vp, C.c_int32, C.c_int32, vp, C.c_int32, C.c_int32, vp, vp]
+    i64, i32 = C.c_int64, C.c_int32
+    lib.mw_paged_plan.argtypes = [C.POINTER(PlanArgs), C.c_int, vp]
+    lib.mw_paged_write.argtypes = [C.POINTER(PagedCache), vp, vp, C.c_int, i64, i64, i64, i64, vp, i64, C.c_int, vp]
+    lib.mw_tree_attention_workspace.argtypes = [C.POINTER(TreeArgs)]
+    lib.mw_tree_attention.argtypes = [C.POINTER(TreeArgs), C.c_int, vp]
+    lib.mw_tree_accept_workspace.argtypes = [C.POINTER(AcceptArgs)]
+    lib.mw_tree_accept.argtypes = [C.POINTER(AcceptArgs), C.c_int, vp]
+    lib.mw_paged_compact.argtypes = [C.POINTER(PagedCache), i32, i64, vp, i64, i32, vp, vp, i32, vp, i32, C.c_int, vp]
+    lib.mw_tree_attention_workspace.restype = lib.mw_tree_accept_workspace.restype = i64
     for name in SYMBOLS:
+        if name.endswith("_workspace"):
+            continue
         if name not in ("mw_destroy", "mw_last_error", "mw_align_destroy", "mw_align_last_error", "mw_align_frames", "mw_sample_uniform"):
             getattr(lib, name).restype = C.c_int
     _lib = lib

@@ -18,6 +18,7 @@
 using namespace mw;
 
 static thread_local std::string g_create_error;
+namespace mw { void set_call_error(const std::string& msg) { g_create_error = msg; } }      // failures of calls without a context
 
 // Scratch of mw_logmel_noalloc, the one entry point that allocates nothing: the per-block maxima of the
 // log-mel kernel (94 floats per chunk, kNoAllocMaxBatch chunks), which mel_norm_kernel reduces to each chunk's

@@ -1,0 +1,562 @@
+// Attention of trees of drafted tokens over a K/V cache in pages, for gfx950.
+//
+// For row (node) i of request b and query head h:  out = sum_j p_j V[j],  p = softmax_j(scale * q . K[j])  over the keys that
+// the row sees: all of the request's `kept` cached tokens, and of its own step's nodes (at positions kept ..) those whose
+// bit is set in the row's mask, or without a mask the nodes up to itself.  A row that sees nothing is zero.
+//
+// Bound: the K/V rows of a request are read once per K/V head for all nodes and all query heads of its group, so a step with
+// few columns (nodes x heads per K/V head) is bound by HBM, one with some hundred of them by the matrix cores.
+//
+// One workgroup takes one work unit (a stretch of a request's keys), one K/V head and up to 128 query columns.  Keys are on
+// the row index of the matrix instructions, so that a lane's scores belong to one query column: S^T = K Q^T, then
+// O^T = V^T P^T with P straight from the registers of S (its 4-key groups are the k-slots of the second product) and
+// V^T by transposing LDS reads.  Tiles of 64 keys go global -> registers -> LDS, the next tile's loads in flight behind the
+// current tile's products.  The softmax is online: one running maximum and sum per column.
+// A request that is cut into several units leaves its partial results (fp32, with maximum and sum) in the workspace and a
+// second launch joins them.
+#include "mw_kernels.h"
+
+namespace mw {
+
+namespace {
+
+typedef __bf16 bf16;
+typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef short short8v __attribute__((ext_vector_type(8)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int KT = 64;                                       // keys of a tile
+
+template <typename T> struct Mat;
+template <> struct Mat<f16> {
+    static __device__ __forceinline__ float4v mma32(short8v a, short8v b, float4v c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ float4v mma16(short4v a, short4v b, float4v c) {
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(half4, a), __builtin_bit_cast(half4, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ bool infinite(unsigned w) { return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u; }
+};
+template <> struct Mat<bf16> {
+    static __device__ __forceinline__ float4v mma32(short8v a, short8v b, float4v c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, a), __builtin_bit_cast(bf8v, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ float4v mma16(short4v a, short4v b, float4v c) {
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ bool infinite(unsigned w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
+};
+template <typename T> __device__ __forceinline__ short bits_of(float x) { return __builtin_bit_cast(short, (T)x); }       // nearest even
+
+__device__ __forceinline__ float column_max(float v) {       // over the four lanes that share a query column
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float column_sum(float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+// LDS images of a tile: rows of D values in chunks of 8; the chunk index is exchanged by the row so that the rows that one
+// instruction reads (16 of K, 8 of V) start in different banks.
+template <int D> __device__ __forceinline__ int k_at(int row, int chunk) {
+    return row * D + ((chunk ^ (D == 64 ? (row >> 1) & 7 : row & 15)) << 3);
+}
+template <int D> __device__ __forceinline__ int v_at(int row, int col) {
+    return row * D + ((((col >> 3) ^ (D == 64 ? ((row >> 1) & 3) << 1 : (row & 7) << 1)) << 3) | (col & 7));
+}
+// 16 e4m3 codes -> 16 values of T (exact)
+template <typename T> __device__ __forceinline__ void widen16(uint4 u, uint4 (&out)[2]) {
+    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+    unsigned short h[16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        const f2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
+        h[4 * i] = (unsigned short)bits_of<T>(lo[0]); h[4 * i + 1] = (unsigned short)bits_of<T>(lo[1]);
+        h[4 * i + 2] = (unsigned short)bits_of<T>(hi[0]); h[4 * i + 3] = (unsigned short)bits_of<T>(hi[1]);
+    }
+    __builtin_memcpy(out, h, 32);
+}
+
+// T: type of q, of the products and of out.  KV8: the cache holds e4m3 codes with a scale per row; the codes go to the matrix
+// cores as they are, K's scale multiplies the score and V's the weight.  QT: 16-column query tiles per wave.  WK: waves that
+// share the columns and split a tile's keys; 4 / WK groups of waves hold different columns.
+template <typename T, bool KV8, int D, int QT, int WK>
+__global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeAttnParams p, int n_blocks, int group) {
+    constexpr int WQ = 4 / WK, NK = 4 / WK, CB = 16 * QT * WQ;
+    constexpr int EPL = KV8 ? 16 : 8;                        // values of a 16-byte load
+    constexpr int CPR = D / EPL, RPP = 256 / CPR, NI = KT / RPP;
+    constexpr int ND = D / 16;
+    __shared__ __attribute__((aligned(16))) short tiles[4 * KT * D];         // K of both buffers, V of both buffers
+    __shared__ __attribute__((aligned(16))) float scales[2][2][KV8 ? KT : 4];
+    __shared__ __attribute__((aligned(16))) int page_ok[2][4];               // per 16 keys: the page exists
+    __shared__ int bad_v[2];                                 // tile + 1 whose V rows of this step hold an infinity or a NaN
+    __shared__ float red_m[4][16 * QT], red_l[4][16 * QT];
+    short* const ldsK = tiles;
+    short* const ldsV = tiles + 2 * KT * D;
+
+    // workgroup -> (unit, K/V head, column block): the blocks of one (unit, head) are 8 ids apart, on the same XCD, so that
+    // its K/V rows come from that XCD's L2 after the first of them
+    const int pair = blockIdx.x / (8 * n_blocks) * 8 + (blockIdx.x & 7), cb = (blockIdx.x >> 3) % n_blocks;
+    const int unit = pair / p.c.heads, g = pair - unit * p.c.heads;
+    if (unit >= p.n_units) return;
+    const int4 work = reinterpret_cast<const int4*>(p.units)[unit];
+    const int b = work.x;
+    if (b < 0 || b >= p.batch) return;
+    const int row0 = max(0, p.row_start[b]);
+    const int nodes = min(min(p.row_start[b + 1], p.rows) - row0, p.max_nodes);
+    const int cols = nodes * group;
+    if (cb * CB >= cols) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int fr = lane & 15, fg = lane >> 4;
+    const int wq = wave / WK, wk = wave % WK;
+    const int kept = max(0, p.kept[b]);
+    // keys of this workgroup: the unit's, none behind the last one that a row of this block can see
+    const int last_node = p.mask ? nodes - 1 : min(nodes - 1, (cb * CB + CB - 1) / group);
+    const int longest = p.max_pages << p.c.page_shift;
+    const int key0 = max(0, work.y) & ~(KT - 1);
+    const int key1 = (int)min((long)min(work.z, longest), (long)kept + last_node + 1);
+    const int n_tiles = key1 > key0 ? (key1 - key0 + KT - 1) / KT : 0;
+
+    // ---- the query columns of this wave
+    short8v qf[QT][D / 32];
+    int node[QT];
+#pragma unroll
+    for (int qs = 0; qs < QT; ++qs) {
+        const int c = min(cb * CB + (wq * QT + qs) * 16 + fr, cols - 1);
+        node[qs] = c / group;
+        const short* src = static_cast<const short*>(p.q) + (long)(row0 + node[qs]) * p.q_row + (long)(g * group + c - node[qs] * group) * p.q_head;
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) qf[qs][s] = *reinterpret_cast<const short8v*>(src + s * 32 + fg * 8);
+    }
+
+    // ---- staging
+    const int ch = tid % CPR, srow = tid / CPR;
+    const int* const pages = p.table + (long)b * p.table_stride;
+    const int page_mask = (1 << p.c.page_shift) - 1;
+    uint4 rk[NI], rv[NI];
+    int pg[NI], pg_s = 0;                                    // pages of the rows to be loaded next
+    unsigned ok = 0;                                         // bit i: row i of the loaded tile exists
+    float rscale = 0.f;
+    auto page_id = [&](int key) -> int { return key < key1 ? pages[key >> p.c.page_shift] : -1; };
+    auto load_pages = [&](int kv0) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) pg[i] = page_id(kv0 + srow + RPP * i);
+        if constexpr (KV8) pg_s = page_id(kv0 + (tid & (KT - 1)));
+    };
+    auto load_tile = [&](int kv0) {
+        ok = 0;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int key = kv0 + srow + RPP * i;
+            const bool there = pg[i] >= 0 && pg[i] < p.c.n_pages;
+            ok |= there ? 1u << i : 0u;
+            const long off = (long)(there ? pg[i] : 0) * p.c.page_stride + g * p.c.head_stride + (long)(key & page_mask) * p.c.token_stride + ch * EPL;
+            if constexpr (KV8) {
+                rk[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.c.k) + off);
+                rv[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.c.v) + off);
+            } else {
+                rk[i] = *reinterpret_cast<const uint4*>(static_cast<const short*>(p.c.k) + off);
+                rv[i] = *reinterpret_cast<const uint4*>(static_cast<const short*>(p.c.v) + off);
+            }
+        }
+        if constexpr (KV8) {
+            if (tid < 2 * KT) {
+                const bool there = pg_s >= 0 && pg_s < p.c.n_pages;
+                const long at = (((long)(there ? pg_s : 0) * p.c.heads + g) << p.c.page_shift) + ((kv0 + (tid & (KT - 1))) & page_mask);
+                rscale = there ? (tid < KT ? p.c.ks : p.c.vs)[at] : 0.f;
+            }
+        }
+    };
+    auto store_tile = [&](int buf, int it) {
+        const bool own_step = key0 + it * KT + KT > kept;    // the tile holds rows of this step: a node may not see some of them
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int row = srow + RPP * i;
+            const bool there = ok >> i & 1;
+            uint4 v = rv[i];
+            if (!there) v = make_uint4(0, 0, 0, 0);          // what lies behind the last key may be anything: weight 0 times NaN is NaN
+            if constexpr (KV8) {
+                uint4 w[2];
+                widen16<T>(rk[i], w);
+                *reinterpret_cast<uint4*>(&ldsK[buf * KT * D + k_at<D>(row, 2 * ch)]) = w[0];
+                *reinterpret_cast<uint4*>(&ldsK[buf * KT * D + k_at<D>(row, 2 * ch + 1)]) = w[1];
+                widen16<T>(v, w);
+                *reinterpret_cast<uint4*>(&ldsV[buf * KT * D + v_at<D>(row, 16 * ch)]) = w[0];
+                *reinterpret_cast<uint4*>(&ldsV[buf * KT * D + v_at<D>(row, 16 * ch + 8)]) = w[1];
+                if (own_step)
+                    bad = bad || Mat<T>::infinite(w[0].x) || Mat<T>::infinite(w[0].y) || Mat<T>::infinite(w[0].z) || Mat<T>::infinite(w[0].w) ||
+                          Mat<T>::infinite(w[1].x) || Mat<T>::infinite(w[1].y) || Mat<T>::infinite(w[1].z) || Mat<T>::infinite(w[1].w);
+            } else {
+                *reinterpret_cast<uint4*>(&ldsK[buf * KT * D + k_at<D>(row, ch)]) = rk[i];
+                *reinterpret_cast<uint4*>(&ldsV[buf * KT * D + v_at<D>(row, 8 * ch)]) = v;
+                if (own_step) bad = bad || Mat<T>::infinite(v.x) || Mat<T>::infinite(v.y) || Mat<T>::infinite(v.z) || Mat<T>::infinite(v.w);
+            }
+            if (ch == 0 && (row & 15) == 0) page_ok[buf][row >> 4] = there;
+        }
+        if (bad) bad_v[buf] = it + 1;
+        if constexpr (KV8) {
+            if (tid < 2 * KT) scales[buf][tid / KT][tid & (KT - 1)] = rscale;
+        }
+    };
+
+    float4v o[ND][QT];                                       // O^T: rows of 16 head dims, columns of 16 queries
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int qs = 0; qs < QT; ++qs) o[d][qs] = float4v{0, 0, 0, 0};
+    float m[QT], l[QT];
+#pragma unroll
+    for (int qs = 0; qs < QT; ++qs) { m[qs] = -INFINITY; l[qs] = 0.f; }
+    // e4m3: weights are p_j times V's row scale relative to a power of two above every scale seen so far, so that they stay
+    // within fp16's range whatever the scales are; the accumulators are multiplied by it at the end
+    float vref = 0.f;
+    const float to_log2 = p.scale * kLog2e;
+
+    if (tid < 2) bad_v[tid] = 0;
+    if (n_tiles > 0) {
+        load_pages(key0);
+        load_tile(key0);
+        load_pages(key0 + KT);
+        __syncthreads();
+        store_tile(0, 0);
+    }
+    __syncthreads();
+    for (int it = 0; it < n_tiles; ++it) {
+        const int buf = it & 1, kv0 = key0 + it * KT;
+        if (it + 1 < n_tiles) {
+            load_tile(kv0 + KT);
+            load_pages(kv0 + 2 * KT);
+        }
+        // ---- S^T
+        float4v sc[NK][QT];
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+            const int krow = (wk * NK + i) * 16 + fr;
+#pragma unroll
+            for (int qs = 0; qs < QT; ++qs) sc[i][qs] = float4v{0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < D / 32; ++s) {
+                const short8v kf = *reinterpret_cast<const short8v*>(&ldsK[buf * KT * D + k_at<D>(krow, s * 4 + fg)]);
+#pragma unroll
+                for (int qs = 0; qs < QT; ++qs) sc[i][qs] = Mat<T>::mma32(kf, qf[qs][s], sc[i][qs]);
+            }
+        }
+        // ---- scores in units of log2; the keys that a column does not see
+        const int4 there = *reinterpret_cast<const int4*>(page_ok[buf]);
+        const bool edge = kv0 + KT > kept || kv0 + KT > key1 || !(there.x && there.y && there.z && there.w);
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+            float4v by = float4v{to_log2, to_log2, to_log2, to_log2};
+            if constexpr (KV8) {
+                const float4v s4 = *reinterpret_cast<const float4v*>(&scales[buf][0][(wk * NK + i) * 16 + 4 * fg]);
+                by = float4v{s4[0] * to_log2, s4[1] * to_log2, s4[2] * to_log2, s4[3] * to_log2};
+            }
+#pragma unroll
+            for (int qs = 0; qs < QT; ++qs)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sc[i][qs][r] *= by[r];
+        }
+        if (edge) {
+            const int first = kv0 - kept, limit = key1 - kv0;                 // node of the tile's first key (may be negative)
+            unsigned long long exist = limit >= 64 ? ~0ull : (1ull << limit) - 1;
+            if (!there.x) exist &= ~0xffffull;
+            if (!there.y) exist &= ~0xffff0000ull;
+            if (!there.z) exist &= ~0xffff00000000ull;
+            if (!there.w) exist &= ~0xffff000000000000ull;
+#pragma unroll
+            for (int qs = 0; qs < QT; ++qs) {
+                unsigned long long sees;                                     // bit k: key kv0 + k
+                if (p.mask) {
+                    const unsigned* words = p.mask + (long)(row0 + node[qs]) * p.mask_words;
+                    auto word = [&](int w) -> unsigned long long { return w >= 0 && w < p.mask_words ? words[w] : 0u; };
+                    if (first <= -64) sees = ~0ull;
+                    else if (first < 0) sees = ((word(0) | word(1) << 32) << -first) | ((1ull << -first) - 1);
+                    else {
+                        const int w = first >> 5, sh = first & 31;
+                        sees = (word(w) | word(w + 1) << 32) >> sh;
+                        if (sh) sees |= word(w + 2) << (64 - sh);
+                    }
+                } else {
+                    const int n = node[qs] - first + 1;
+                    sees = n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
+                }
+                sees &= exist;
+#pragma unroll
+                for (int i = 0; i < NK; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (!(sees >> ((wk * NK + i) * 16 + 4 * fg + r) & 1)) sc[i][qs][r] = -INFINITY;
+            }
+        }
+        // ---- online softmax
+        float mn[QT];
+        bool lift = false;
+#pragma unroll
+        for (int qs = 0; qs < QT; ++qs) {
+            float x = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < NK; ++i) x = fmaxf(x, fmaxf(fmaxf(sc[i][qs][0], sc[i][qs][1]), fmaxf(sc[i][qs][2], sc[i][qs][3])));
+            mn[qs] = fmaxf(m[qs], column_max(x));
+            lift = lift || mn[qs] > m[qs];
+        }
+        if (__any(lift)) {
+#pragma unroll
+            for (int qs = 0; qs < QT; ++qs) {
+                const float alpha = mn[qs] > m[qs] ? __builtin_amdgcn_exp2f(m[qs] - mn[qs]) : 1.f;
+                m[qs] = mn[qs];
+                l[qs] *= alpha;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) { o[d][qs][0] *= alpha; o[d][qs][1] *= alpha; o[d][qs][2] *= alpha; o[d][qs][3] *= alpha; }
+            }
+        }
+        float vinv = 0.f;
+        if constexpr (KV8) {
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < NK; ++i) {
+                const float4v s4 = *reinterpret_cast<const float4v*>(&scales[buf][1][(wk * NK + i) * 16 + 4 * fg]);
+                top = fmaxf(top, fmaxf(fmaxf(s4[0], s4[1]), fmaxf(s4[2], s4[3])));
+            }
+            top = column_max(top);
+            if (top > vref) {                                // the same in all lanes
+                const float up = __uint_as_float(min((__float_as_uint(top) & 0x7f800000u) + 0x00800000u, 0x7f000000u));
+                const float f = vref / up;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int qs = 0; qs < QT; ++qs) { o[d][qs][0] *= f; o[d][qs][1] *= f; o[d][qs][2] *= f; o[d][qs][3] *= f; }
+                vref = up;
+            }
+            vinv = vref > 0.f ? 1.f / vref : 0.f;
+        }
+#pragma unroll
+        for (int qs = 0; qs < QT; ++qs) {
+            const float ref = m[qs] == -INFINITY ? 0.f : m[qs];               // nothing seen yet: every weight is 0
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < NK; ++i) {
+                float4v vs4 = float4v{1, 1, 1, 1};
+                if constexpr (KV8) vs4 = *reinterpret_cast<const float4v*>(&scales[buf][1][(wk * NK + i) * 16 + 4 * fg]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float w = __builtin_amdgcn_exp2f(sc[i][qs][r] - ref);
+                    sum += w;
+                    if constexpr (KV8) sc[i][qs][r] = edge && w == 0.f ? 0.f : w * (vs4[r] * vinv);
+                    else sc[i][qs][r] = w;
+                }
+            }
+            l[qs] += sum;                                    // of this lane's keys; the column's sum is formed at the end
+        }
+        // ---- O^T += V^T P^T.  The weights are rounded once to T (half a step of T each, as the result is); the sum above is of
+        // the unrounded ones.
+        const short* const vt = ldsV + buf * KT * D;
+        if (bad_v[buf] == it + 1) {
+            // a value of this step's rows is no number: every key for itself, so that it reaches only the rows that see it
+            for (int kk = 0; kk < NK * 16; ++kk) {
+                const int key = wk * NK * 16 + kk;
+#pragma unroll
+                for (int qs = 0; qs < QT; ++qs) {
+                    float mine = 0.f;
+#pragma unroll
+                    for (int i = 0; i < NK; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if ((kk >> 4) == i && (kk & 3) == r) mine = sc[i][qs][r];
+                    const float w = __shfl(mine, fr + 16 * ((kk >> 2) & 3));
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        const short4v v4 = *reinterpret_cast<const short4v*>(&vt[v_at<D>(key, d * 16 + 4 * fg)]);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (w != 0.f) o[d][qs][r] += w * (float)__builtin_bit_cast(T, (short)v4[r]);
+                    }
+                }
+            }
+        } else {
+            typedef short4v __attribute__((address_space(3)))* lds4;
+            if constexpr (NK == 1) {
+                short4v pf[QT];
+#pragma unroll
+                for (int qs = 0; qs < QT; ++qs)
+                    pf[qs] = short4v{bits_of<T>(sc[0][qs][0]), bits_of<T>(sc[0][qs][1]), bits_of<T>(sc[0][qs][2]), bits_of<T>(sc[0][qs][3])};
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    const short4v vf = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vt + v_at<D>(wk * 16 + 4 * fg + (fr >> 2), d * 16 + 4 * (fr & 3))));
+#pragma unroll
+                    for (int qs = 0; qs < QT; ++qs) o[d][qs] = Mat<T>::mma16(vf, pf[qs], o[d][qs]);
+                }
+            } else {
+                short8v pf[QT][NK / 2 ? NK / 2 : 1];
+#pragma unroll
+                for (int qs = 0; qs < QT; ++qs)
+#pragma unroll
+                    for (int s = 0; s < NK / 2; ++s)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            pf[qs][s][r] = bits_of<T>(sc[2 * s][qs][r]);
+                            pf[qs][s][4 + r] = bits_of<T>(sc[2 * s + 1][qs][r]);
+                        }
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int s = 0; s < NK / 2; ++s) {       // element j of step s is key 32 s + 16 (j >> 2) + 4 fg + (j & 3) of the wave's
+                        const int krow = wk * NK * 16 + 32 * s + 4 * fg + (fr >> 2);
+                        const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vt + v_at<D>(krow, d * 16 + 4 * (fr & 3))));
+                        const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vt + v_at<D>(krow + 16, d * 16 + 4 * (fr & 3))));
+                        const short8v vf = short8v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+                        for (int qs = 0; qs < QT; ++qs) o[d][qs] = Mat<T>::mma32(vf, pf[qs][s], o[d][qs]);
+                    }
+            }
+        }
+        if (it + 1 < n_tiles) store_tile(buf ^ 1, it + 1);
+        __syncthreads();
+    }
+
+    // ---- join the waves that split the keys, then normalise and store, or leave the partial result to the second launch
+#pragma unroll
+    for (int qs = 0; qs < QT; ++qs) {
+        l[qs] = column_sum(l[qs]);
+        if constexpr (KV8)
+#pragma unroll
+            for (int d = 0; d < ND; ++d) { o[d][qs][0] *= vref; o[d][qs][1] *= vref; o[d][qs][2] *= vref; o[d][qs][3] *= vref; }
+    }
+    if constexpr (WK > 1) {
+        if (fg == 0)
+#pragma unroll
+            for (int qs = 0; qs < QT; ++qs) { red_m[wave][qs * 16 + fr] = m[qs]; red_l[wave][qs * 16 + fr] = l[qs]; }
+        __syncthreads();
+#pragma unroll
+        for (int qs = 0; qs < QT; ++qs) {
+            float all = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < WK; ++w) all = fmaxf(all, red_m[wq * WK + w][qs * 16 + fr]);
+            const float ref = all == -INFINITY ? 0.f : all;
+#pragma unroll
+            for (int w = 0; w < WK; ++w) sum += red_l[wq * WK + w][qs * 16 + fr] * __builtin_amdgcn_exp2f(red_m[wq * WK + w][qs * 16 + fr] - ref);
+            const float f = __builtin_amdgcn_exp2f(m[qs] - ref);
+            m[qs] = all; l[qs] = sum;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) { o[d][qs][0] *= f; o[d][qs][1] *= f; o[d][qs][2] *= f; o[d][qs][3] *= f; }
+        }
+        // a wave's O as [columns][D] floats; wave w of the group adds up the columns' dims [w * D / WK, ...)
+        float* const ex = reinterpret_cast<float*>(tiles);
+        constexpr int WCOLS = 16 * QT;
+#pragma unroll
+        for (int qs = 0; qs < QT; ++qs)
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+                *reinterpret_cast<float4v*>(&ex[((wave * WCOLS) + qs * 16 + fr) * D + (((d * 4 + fg) ^ fr) & (D / 4 - 1)) * 4]) = o[d][qs];
+        __syncthreads();
+        constexpr int DW = ND / WK;                          // 16-dim tiles that a wave adds up
+#pragma unroll
+        for (int qs = 0; qs < QT; ++qs)
+#pragma unroll
+            for (int d = 0; d < DW; ++d) {
+                float4v t = float4v{0, 0, 0, 0};
+#pragma unroll
+                for (int w = 0; w < WK; ++w) {
+                    const float4v x = *reinterpret_cast<const float4v*>(
+                        &ex[(((wq * WK + w) * WCOLS) + qs * 16 + fr) * D + ((((wk * DW + d) * 4 + fg) ^ fr) & (D / 4 - 1)) * 4]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) t[r] += x[r];
+                }
+                o[d][qs] = t;
+            }
+    }
+    constexpr int DW = ND / WK;
+    const int d0 = WK > 1 ? wk * DW : 0;
+#pragma unroll
+    for (int qs = 0; qs < QT; ++qs) {
+        const int c = cb * CB + (wq * QT + qs) * 16 + fr;
+        if (c >= cols) continue;
+        if (work.w <= 1 || !p.workspace) {
+            const float inv = l[qs] == 0.f ? 0.f : 1.f / l[qs];               // (a NaN sum stays NaN)
+            short* dst = static_cast<short*>(p.out) + (long)(row0 + node[qs]) * p.out_row + (long)(g * group + c - node[qs] * group) * p.out_head;
+#pragma unroll
+            for (int d = 0; d < DW; ++d)
+                *reinterpret_cast<short4v*>(dst + (d0 + d) * 16 + 4 * fg) =
+                    short4v{bits_of<T>(o[d][qs][0] * inv), bits_of<T>(o[d][qs][1] * inv), bits_of<T>(o[d][qs][2] * inv), bits_of<T>(o[d][qs][3] * inv)};
+        } else {
+            const long slot = ((long)unit * p.c.heads + g) * (p.max_nodes * group) + c;
+            float* po = p.workspace + slot * D;
+#pragma unroll
+            for (int d = 0; d < DW; ++d) *reinterpret_cast<float4v*>(po + (d0 + d) * 16 + 4 * fg) = o[d][qs];
+            if (fg == 0 && wk == 0) {
+                float* ml = p.workspace + (long)p.n_units * p.c.heads * (p.max_nodes * group) * D + slot * 2;
+                ml[0] = m[qs]; ml[1] = l[qs];
+            }
+        }
+    }
+}
+
+// Rows of requests that were cut: the units' partial results, weighted by their maxima.  One workgroup per (request, node).
+template <typename T, int D>
+__global__ __launch_bounds__(256) void tree_join_kernel(TreeAttnParams p, int group) {
+    const int b = blockIdx.x / p.max_nodes, i = blockIdx.x - b * p.max_nodes;
+    const int u0 = p.unit_start[b], n = p.unit_start[b + 1] - u0;
+    const int row = p.row_start[b] + i;
+    if (n < 2 || u0 < 0 || u0 + n > p.n_units || p.row_start[b] < 0 || row >= p.row_start[b + 1] || row >= p.rows) return;
+    const long cols = (long)p.max_nodes * group;
+    const float* const all_ml = p.workspace + (long)p.n_units * p.c.heads * cols * D;
+    for (int e = threadIdx.x; e < p.heads * (D / 4); e += 256) {
+        const int h = e / (D / 4), d = (e - h * (D / 4)) * 4;
+        const int g = h / group;
+        const long c = (long)i * group + (h - g * group);
+        float top = -INFINITY;
+        for (int u = 0; u < n; ++u) top = fmaxf(top, all_ml[(((long)(u0 + u) * p.c.heads + g) * cols + c) * 2]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float4v acc = float4v{0, 0, 0, 0};
+        float sum = 0.f;
+        for (int u = 0; u < n; ++u) {
+            const long slot = ((long)(u0 + u) * p.c.heads + g) * cols + c;
+            const float f = __builtin_amdgcn_exp2f(all_ml[slot * 2] - ref);
+            sum += f * all_ml[slot * 2 + 1];
+            const float4v x = *reinterpret_cast<const float4v*>(p.workspace + slot * D + d);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[r] += f * x[r];
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        *reinterpret_cast<short4v*>(static_cast<short*>(p.out) + (long)row * p.out_row + (long)h * p.out_head + d) =
+            short4v{bits_of<T>(acc[0] * inv), bits_of<T>(acc[1] * inv), bits_of<T>(acc[2] * inv), bits_of<T>(acc[3] * inv)};
+    }
+}
+
+template <typename T, bool KV8, int D>
+void launch_tree_t(const TreeAttnParams& p, hipStream_t s) {
+    const int group = p.heads / p.c.heads;
+    const long cols = (long)p.max_nodes * group;
+    const int block = cols <= 16 ? 16 : cols <= 32 ? 32 : cols <= 64 ? 64 : 128;
+    const int n_blocks = (int)((cols + block - 1) / block);
+    const long pairs = ((long)p.n_units * p.c.heads + 7) / 8 * 8;
+    const unsigned grid = (unsigned)(pairs * n_blocks);
+    if (block == 16) tree_attn_kernel<T, KV8, D, 1, 4><<<grid, 256, 0, s>>>(p, n_blocks, group);
+    else if (block == 32) tree_attn_kernel<T, KV8, D, 2, 4><<<grid, 256, 0, s>>>(p, n_blocks, group);
+    else if (block == 64) tree_attn_kernel<T, KV8, D, 2, 2><<<grid, 256, 0, s>>>(p, n_blocks, group);
+    else tree_attn_kernel<T, KV8, D, 2, 1><<<grid, 256, 0, s>>>(p, n_blocks, group);
+    if (p.n_units > p.batch) tree_join_kernel<T, D><<<(unsigned)((long)p.batch * p.max_nodes), 256, 0, s>>>(p, group);
+}
+
+}  // namespace
+
+// Partial results of every unit; none where there are no more units than requests (no request is cut then).
+long tree_attn_workspace(int n_units, int batch, int kv_heads, int group, int max_nodes, int dim) {
+    return n_units > batch ? (long)n_units * kv_heads * max_nodes * group * (dim + 2) * 4 : 0;
+}
+
+void launch_tree_attention(const TreeAttnParams& p, hipStream_t s) {
+    if (!p.n_units || !p.batch || !p.max_nodes) return;
+    const bool kv8 = p.c.ks != nullptr;
+    if (p.dim == 64) {
+        if (p.bf16) { if (kv8) launch_tree_t<bf16, true, 64>(p, s); else launch_tree_t<bf16, false, 64>(p, s); }
+        else { if (kv8) launch_tree_t<f16, true, 64>(p, s); else launch_tree_t<f16, false, 64>(p, s); }
+    } else {
+        if (p.bf16) { if (kv8) launch_tree_t<bf16, true, 128>(p, s); else launch_tree_t<bf16, false, 128>(p, s); }
+        else { if (kv8) launch_tree_t<f16, true, 128>(p, s); else launch_tree_t<f16, false, 128>(p, s); }
+    }
+}
+
+}  // namespace mw

@@ -293,4 +293,58 @@ void launch_log_softmax_rows(float* z, int rows, int ld, int V, hipStream_t s);
 // out [rows][1 + J]: column 0 = z[r][blank], column 1 + j = z[r][tokens[j]], or for tokens[j] == -1 the largest z[r][v], v != blank
 void launch_ctc_gather(const float* z, int rows, int ld, int V, const int32_t* tokens, int J, int blank, float* out, hipStream_t s);
 
+// ---------------------------------------------------------------- drafted tokens over a K/V cache in pages
+// One layer of a cache in pages: row (page, head, offset) of K lies at k + page * page_stride + head * head_stride + offset *
+// token_stride elements (V likewise); 16-bit values, or e4m3 codes with one scale per row, ks / vs [page][head][1 << page_shift].
+struct PagedCacheView {
+    void* k; void* v;
+    float* ks; float* vs;                       // null: 16-bit values
+    long page_stride, head_stride, token_stride;
+    int n_pages, page_shift, heads;
+};
+constexpr int kPlanMaxBatch = 2048, kPlanMaxWords = 8;         // requests of a plan; nodes of a tree / 32
+struct PlanParams {
+    int batch, rows, page_shift, max_pages, n_pages;
+    const int *kept, *fresh, *parents;          // parents null: chains
+    int* table; long table_stride;
+    const int* pages_in; int* pages_out;        // [batch], two arrays
+    int* free_list; const int* n_free_in; int* n_free_out;
+    int *row_start, *admitted, *positions;
+    long* slots;
+    unsigned* mask; int mask_words;
+    int* units; int* unit_start; int chunk_units, chunk_min;   // units null: none wanted
+};
+void launch_paged_plan(const PlanParams& p, hipStream_t s);
+// k, v [rows][heads][dim] 16-bit (bf16: bfloat16, else fp16; a 16-bit cache holds the same type); strides in elements
+void launch_paged_write(const PagedCacheView& c, int dim, int bf16, const void* k, const void* v, long k_row, long k_head, long v_row,
+                        long v_head, const long* slots, long rows, hipStream_t s);
+constexpr int kAcceptMaxNodes = 1024, kAcceptMaxParts = 64;
+struct AcceptParams {
+    const void* logits; long stride; int dtype;                // 0 = float32, 1 = fp16, 2 = bfloat16
+    int rows, vocab, batch, depth;
+    const uint8_t* suppress;                                   // [vocab] or null
+    const int *tokens, *parents, *row_start;
+    int *best, *path, *count, *out_tokens;
+    void* workspace;                                           // rows * accept_parts() * 8 bytes
+};
+int accept_parts(long rows, int vocab);
+void launch_tree_accept(const AcceptParams& p, hipStream_t s);
+void launch_paged_compact(const PagedCacheView& c, int layers, long layer_stride, long scale_layer_stride, int dim, const int* table,
+                          long table_stride, int max_pages, const int* kept, const int* path, int path_cols, const int* count, int batch,
+                          hipStream_t s);
+struct TreeAttnParams {
+    PagedCacheView c;
+    int dim, bf16, heads, rows, batch, max_nodes;
+    const void* q; long q_row, q_head;
+    void* out; long out_row, out_head;
+    const int* table; long table_stride; int max_pages;
+    const int *kept, *row_start, *units, *unit_start;
+    int n_units;
+    const unsigned* mask; int mask_words;                      // null: chains
+    float scale;
+    float* workspace;                                          // tree_attn_workspace() bytes; not read when no request is cut
+};
+long tree_attn_workspace(int n_units, int batch, int kv_heads, int group, int max_nodes, int dim);
+void launch_tree_attention(const TreeAttnParams& p, hipStream_t s);
+
 }  // namespace mw
