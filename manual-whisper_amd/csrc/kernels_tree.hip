@@ -24,6 +24,7 @@ typedef __bf16 bf16;
 typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef short short8v __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int KT = 64;                                       // keys of a tile
@@ -36,7 +37,7 @@ template <> struct Mat<f16> {
     static __device__ __forceinline__ float4v mma16(short4v a, short4v b, float4v c) {
         return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(half4, a), __builtin_bit_cast(half4, b), c, 0, 0, 0);
     }
-    static __device__ __forceinline__ bool infinite(unsigned w) { return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u; }
+    static constexpr unsigned kExp = 0x7c007c00u;            // exponents of a pair of values
 };
 template <> struct Mat<bf16> {
     static __device__ __forceinline__ float4v mma32(short8v a, short8v b, float4v c) {
@@ -45,8 +46,19 @@ template <> struct Mat<bf16> {
     static __device__ __forceinline__ float4v mma16(short4v a, short4v b, float4v c) {
         return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
     }
-    static __device__ __forceinline__ bool infinite(unsigned w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
+    static constexpr unsigned kExp = 0x7f807f80u;
 };
+// eight values with 0 in the place of infinities and NaN (all bits of the exponent set); `any`: whether there were some
+template <typename T> __device__ __forceinline__ u32x4 finite_only(u32x4 u, bool& any) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned e = u[i] & Mat<T>::kExp;
+        const bool lo = (e & 0xffffu) == (Mat<T>::kExp & 0xffffu), hi = (e >> 16) == (Mat<T>::kExp >> 16);
+        u[i] &= (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0x0000ffffu : 0xffffffffu);
+        any = any || lo || hi;
+    }
+    return u;
+}
 template <typename T> __device__ __forceinline__ short bits_of(float x) { return __builtin_bit_cast(short, (T)x); }       // nearest even
 
 __device__ __forceinline__ float column_max(float v) {       // over the four lanes that share a query column
@@ -65,36 +77,33 @@ template <int D> __device__ __forceinline__ int k_at(int row, int chunk) {
 template <int D> __device__ __forceinline__ int v_at(int row, int col) {
     return row * D + ((((col >> 3) ^ (D == 64 ? ((row >> 1) & 3) << 1 : (row & 7) << 1)) << 3) | (col & 7));
 }
-// 16 e4m3 codes -> 16 values of T (exact)
-template <typename T> __device__ __forceinline__ void widen16(uint4 u, uint4 (&out)[2]) {
-    const unsigned w[4] = {u.x, u.y, u.z, u.w};
-    unsigned short h[16];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        typedef float f2 __attribute__((ext_vector_type(2)));
-        const f2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
-        h[4 * i] = (unsigned short)bits_of<T>(lo[0]); h[4 * i + 1] = (unsigned short)bits_of<T>(lo[1]);
-        h[4 * i + 2] = (unsigned short)bits_of<T>(hi[0]); h[4 * i + 3] = (unsigned short)bits_of<T>(hi[1]);
-    }
-    __builtin_memcpy(out, h, 32);
+// 8 e4m3 codes -> 8 values of T (exact)
+template <typename T> __device__ __forceinline__ short8v widen8(unsigned a, unsigned b) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const f2 x0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)a, false), x1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)a, true);
+    const f2 x2 = __builtin_amdgcn_cvt_pk_f32_fp8((int)b, false), x3 = __builtin_amdgcn_cvt_pk_f32_fp8((int)b, true);
+    return short8v{bits_of<T>(x0[0]), bits_of<T>(x0[1]), bits_of<T>(x1[0]), bits_of<T>(x1[1]),
+                   bits_of<T>(x2[0]), bits_of<T>(x2[1]), bits_of<T>(x3[0]), bits_of<T>(x3[1])};
 }
 
 // T: type of q, of the products and of out.  KV8: the cache holds e4m3 codes with a scale per row; the codes go to the matrix
 // cores as they are, K's scale multiplies the score and V's the weight.  QT: 16-column query tiles per wave.  WK: waves that
 // share the columns and split a tile's keys; 4 / WK groups of waves hold different columns.
 template <typename T, bool KV8, int D, int QT, int WK>
-__global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeAttnParams p, int n_blocks, int group) {
+__global__ __launch_bounds__(256, QT == 1 ? (D == 64 ? 4 : 3) : 2) void tree_attn_kernel(TreeAttnParams p, int n_blocks, int group) {
     constexpr int WQ = 4 / WK, NK = 4 / WK, CB = 16 * QT * WQ;
     constexpr int EPL = KV8 ? 16 : 8;                        // values of a 16-byte load
     constexpr int CPR = D / EPL, RPP = 256 / CPR, NI = KT / RPP;
     constexpr int ND = D / 16;
-    __shared__ __attribute__((aligned(16))) short tiles[4 * KT * D];         // K of both buffers, V of both buffers
-    __shared__ __attribute__((aligned(16))) float scales[2][2][KV8 ? KT : 4];
-    __shared__ __attribute__((aligned(16))) int page_ok[2][4];               // per 16 keys: the page exists
-    __shared__ int bad_v[2];                                 // tile + 1 whose V rows of this step hold an infinity or a NaN
+    // K and V of a tile; at the end the partial results of the waves that split the keys
+    constexpr int kTile = 2 * KT * D, kJoin = WK > 1 ? 2 * 4 * 16 * QT * D : 0;
+    __shared__ __attribute__((aligned(16))) short tiles[kTile > kJoin ? kTile : kJoin];
+    __shared__ __attribute__((aligned(16))) float scales[2][KV8 ? KT : 4];
+    __shared__ __attribute__((aligned(16))) int page_ok[4];  // per 16 keys: the page exists
+    __shared__ int bad_v;                                    // V rows of this step held an infinity or a NaN
     __shared__ float red_m[4][16 * QT], red_l[4][16 * QT];
     short* const ldsK = tiles;
-    short* const ldsV = tiles + 2 * KT * D;
+    short* const ldsV = tiles + KT * D;
 
     // workgroup -> (unit, K/V head, column block): the blocks of one (unit, head) are 8 ids apart, on the same XCD, so that
     // its K/V rows come from that XCD's L2 after the first of them
@@ -135,7 +144,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeAttnParams p, int
     const int ch = tid % CPR, srow = tid / CPR;
     const int* const pages = p.table + (long)b * p.table_stride;
     const int page_mask = (1 << p.c.page_shift) - 1;
-    uint4 rk[NI], rv[NI];
+    u32x4 rk[NI], rv[NI];
     int pg[NI], pg_s = 0;                                    // pages of the rows to be loaded next
     unsigned ok = 0;                                         // bit i: row i of the loaded tile exists
     float rscale = 0.f;
@@ -154,11 +163,11 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeAttnParams p, int
             ok |= there ? 1u << i : 0u;
             const long off = (long)(there ? pg[i] : 0) * p.c.page_stride + g * p.c.head_stride + (long)(key & page_mask) * p.c.token_stride + ch * EPL;
             if constexpr (KV8) {
-                rk[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.c.k) + off);
-                rv[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.c.v) + off);
+                rk[i] = *reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(p.c.k) + off);
+                rv[i] = *reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(p.c.v) + off);
             } else {
-                rk[i] = *reinterpret_cast<const uint4*>(static_cast<const short*>(p.c.k) + off);
-                rv[i] = *reinterpret_cast<const uint4*>(static_cast<const short*>(p.c.v) + off);
+                rk[i] = *reinterpret_cast<const u32x4*>(static_cast<const short*>(p.c.k) + off);
+                rv[i] = *reinterpret_cast<const u32x4*>(static_cast<const short*>(p.c.v) + off);
             }
         }
         if constexpr (KV8) {
@@ -169,36 +178,33 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeAttnParams p, int
             }
         }
     };
-    auto store_tile = [&](int buf, int it) {
-        const bool own_step = key0 + it * KT + KT > kept;    // the tile holds rows of this step: a node may not see some of them
+    auto store_tile = [&](int it) {
+        // In tiles with rows of this step V's infinities and NaN are held back: in the product they would reach rows that do not
+        // see them (0 times NaN is NaN).  The rows that do get them at the end.
+        const bool own_step = key0 + it * KT + KT > kept;
         bool bad = false;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int row = srow + RPP * i;
             const bool there = ok >> i & 1;
-            uint4 v = rv[i];
-            if (!there) v = make_uint4(0, 0, 0, 0);          // what lies behind the last key may be anything: weight 0 times NaN is NaN
+            const u32x4 none = {0, 0, 0, 0};
+            const u32x4 v = there ? rv[i] : none;            // what lies behind the last key may be anything
             if constexpr (KV8) {
-                uint4 w[2];
-                widen16<T>(rk[i], w);
-                *reinterpret_cast<uint4*>(&ldsK[buf * KT * D + k_at<D>(row, 2 * ch)]) = w[0];
-                *reinterpret_cast<uint4*>(&ldsK[buf * KT * D + k_at<D>(row, 2 * ch + 1)]) = w[1];
-                widen16<T>(v, w);
-                *reinterpret_cast<uint4*>(&ldsV[buf * KT * D + v_at<D>(row, 16 * ch)]) = w[0];
-                *reinterpret_cast<uint4*>(&ldsV[buf * KT * D + v_at<D>(row, 16 * ch + 8)]) = w[1];
-                if (own_step)
-                    bad = bad || Mat<T>::infinite(w[0].x) || Mat<T>::infinite(w[0].y) || Mat<T>::infinite(w[0].z) || Mat<T>::infinite(w[0].w) ||
-                          Mat<T>::infinite(w[1].x) || Mat<T>::infinite(w[1].y) || Mat<T>::infinite(w[1].z) || Mat<T>::infinite(w[1].w);
+                *reinterpret_cast<short8v*>(&ldsK[k_at<D>(row, 2 * ch)]) = widen8<T>(rk[i][0], rk[i][1]);
+                *reinterpret_cast<short8v*>(&ldsK[k_at<D>(row, 2 * ch + 1)]) = widen8<T>(rk[i][2], rk[i][3]);
+                u32x4 lo = __builtin_bit_cast(u32x4, widen8<T>(v[0], v[1])), hi = __builtin_bit_cast(u32x4, widen8<T>(v[2], v[3]));
+                if (own_step) { lo = finite_only<T>(lo, bad); hi = finite_only<T>(hi, bad); }
+                *reinterpret_cast<u32x4*>(&ldsV[v_at<D>(row, 16 * ch)]) = lo;
+                *reinterpret_cast<u32x4*>(&ldsV[v_at<D>(row, 16 * ch + 8)]) = hi;
             } else {
-                *reinterpret_cast<uint4*>(&ldsK[buf * KT * D + k_at<D>(row, ch)]) = rk[i];
-                *reinterpret_cast<uint4*>(&ldsV[buf * KT * D + v_at<D>(row, 8 * ch)]) = v;
-                if (own_step) bad = bad || Mat<T>::infinite(v.x) || Mat<T>::infinite(v.y) || Mat<T>::infinite(v.z) || Mat<T>::infinite(v.w);
+                *reinterpret_cast<u32x4*>(&ldsK[k_at<D>(row, ch)]) = rk[i];
+                *reinterpret_cast<u32x4*>(&ldsV[v_at<D>(row, 8 * ch)]) = own_step ? finite_only<T>(v, bad) : v;
             }
-            if (ch == 0 && (row & 15) == 0) page_ok[buf][row >> 4] = there;
+            if (ch == 0 && (row & 15) == 0) page_ok[row >> 4] = there;
         }
-        if (bad) bad_v[buf] = it + 1;
+        if (bad) bad_v = 1;
         if constexpr (KV8) {
-            if (tid < 2 * KT) scales[buf][tid / KT][tid & (KT - 1)] = rscale;
+            if (tid < 2 * KT) scales[tid / KT][tid & (KT - 1)] = rscale;
         }
     };
 
@@ -215,17 +221,31 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeAttnParams p, int
     float vref = 0.f;
     const float to_log2 = p.scale * kLog2e;
 
-    if (tid < 2) bad_v[tid] = 0;
+    // which of the 64 keys from node `first` on (negative: kept tokens before it) the row of node `n` sees
+    auto visible = [&](int n, int first) -> unsigned long long {
+        if (first <= -64) return ~0ull;
+        if (!p.mask) {
+            const int c = n - first + 1;
+            return c <= 0 ? 0ull : c >= 64 ? ~0ull : (1ull << c) - 1;
+        }
+        const unsigned* words = p.mask + (long)(row0 + n) * p.mask_words;
+        auto word = [&](int w) -> unsigned long long { return w < p.mask_words ? words[w] : 0u; };
+        if (first < 0) return ((word(0) | word(1) << 32) << -first) | ((1ull << -first) - 1);
+        const int w = first >> 5, sh = first & 31;
+        const unsigned long long x = (word(w) | word(w + 1) << 32) >> sh;
+        return sh ? x | word(w + 2) << (64 - sh) : x;
+    };
+    if (tid == 0) bad_v = 0;
     if (n_tiles > 0) {
         load_pages(key0);
         load_tile(key0);
         load_pages(key0 + KT);
-        __syncthreads();
-        store_tile(0, 0);
     }
-    __syncthreads();
     for (int it = 0; it < n_tiles; ++it) {
-        const int buf = it & 1, kv0 = key0 + it * KT;
+        const int kv0 = key0 + it * KT;
+        __syncthreads();                                     // the previous tile has been read
+        store_tile(it);
+        __syncthreads();
         if (it + 1 < n_tiles) {
             load_tile(kv0 + KT);
             load_pages(kv0 + 2 * KT);
@@ -239,19 +259,19 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeAttnParams p, int
             for (int qs = 0; qs < QT; ++qs) sc[i][qs] = float4v{0, 0, 0, 0};
 #pragma unroll
             for (int s = 0; s < D / 32; ++s) {
-                const short8v kf = *reinterpret_cast<const short8v*>(&ldsK[buf * KT * D + k_at<D>(krow, s * 4 + fg)]);
+                const short8v kf = *reinterpret_cast<const short8v*>(&ldsK[k_at<D>(krow, s * 4 + fg)]);
 #pragma unroll
                 for (int qs = 0; qs < QT; ++qs) sc[i][qs] = Mat<T>::mma32(kf, qf[qs][s], sc[i][qs]);
             }
         }
         // ---- scores in units of log2; the keys that a column does not see
-        const int4 there = *reinterpret_cast<const int4*>(page_ok[buf]);
+        const int4 there = *reinterpret_cast<const int4*>(page_ok);
         const bool edge = kv0 + KT > kept || kv0 + KT > key1 || !(there.x && there.y && there.z && there.w);
 #pragma unroll
         for (int i = 0; i < NK; ++i) {
             float4v by = float4v{to_log2, to_log2, to_log2, to_log2};
             if constexpr (KV8) {
-                const float4v s4 = *reinterpret_cast<const float4v*>(&scales[buf][0][(wk * NK + i) * 16 + 4 * fg]);
+                const float4v s4 = *reinterpret_cast<const float4v*>(&scales[0][(wk * NK + i) * 16 + 4 * fg]);
                 by = float4v{s4[0] * to_log2, s4[1] * to_log2, s4[2] * to_log2, s4[3] * to_log2};
             }
 #pragma unroll
@@ -268,22 +288,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeAttnParams p, int
             if (!there.w) exist &= ~0xffff000000000000ull;
 #pragma unroll
             for (int qs = 0; qs < QT; ++qs) {
-                unsigned long long sees;                                     // bit k: key kv0 + k
-                if (p.mask) {
-                    const unsigned* words = p.mask + (long)(row0 + node[qs]) * p.mask_words;
-                    auto word = [&](int w) -> unsigned long long { return w >= 0 && w < p.mask_words ? words[w] : 0u; };
-                    if (first <= -64) sees = ~0ull;
-                    else if (first < 0) sees = ((word(0) | word(1) << 32) << -first) | ((1ull << -first) - 1);
-                    else {
-                        const int w = first >> 5, sh = first & 31;
-                        sees = (word(w) | word(w + 1) << 32) >> sh;
-                        if (sh) sees |= word(w + 2) << (64 - sh);
-                    }
-                } else {
-                    const int n = node[qs] - first + 1;
-                    sees = n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
-                }
-                sees &= exist;
+                const unsigned long long sees = visible(node[qs], first) & exist;
 #pragma unroll
                 for (int i = 0; i < NK; ++i)
 #pragma unroll
@@ -317,7 +322,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeAttnParams p, int
             float top = 0.f;
 #pragma unroll
             for (int i = 0; i < NK; ++i) {
-                const float4v s4 = *reinterpret_cast<const float4v*>(&scales[buf][1][(wk * NK + i) * 16 + 4 * fg]);
+                const float4v s4 = *reinterpret_cast<const float4v*>(&scales[1][(wk * NK + i) * 16 + 4 * fg]);
                 top = fmaxf(top, fmaxf(fmaxf(s4[0], s4[1]), fmaxf(s4[2], s4[3])));
             }
             top = column_max(top);
@@ -339,7 +344,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeAttnParams p, int
 #pragma unroll
             for (int i = 0; i < NK; ++i) {
                 float4v vs4 = float4v{1, 1, 1, 1};
-                if constexpr (KV8) vs4 = *reinterpret_cast<const float4v*>(&scales[buf][1][(wk * NK + i) * 16 + 4 * fg]);
+                if constexpr (KV8) vs4 = *reinterpret_cast<const float4v*>(&scales[1][(wk * NK + i) * 16 + 4 * fg]);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const float w = __builtin_amdgcn_exp2f(sc[i][qs][r] - ref);
@@ -352,30 +357,8 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeAttnParams p, int
         }
         // ---- O^T += V^T P^T.  The weights are rounded once to T (half a step of T each, as the result is); the sum above is of
         // the unrounded ones.
-        const short* const vt = ldsV + buf * KT * D;
-        if (bad_v[buf] == it + 1) {
-            // a value of this step's rows is no number: every key for itself, so that it reaches only the rows that see it
-            for (int kk = 0; kk < NK * 16; ++kk) {
-                const int key = wk * NK * 16 + kk;
-#pragma unroll
-                for (int qs = 0; qs < QT; ++qs) {
-                    float mine = 0.f;
-#pragma unroll
-                    for (int i = 0; i < NK; ++i)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if ((kk >> 4) == i && (kk & 3) == r) mine = sc[i][qs][r];
-                    const float w = __shfl(mine, fr + 16 * ((kk >> 2) & 3));
-#pragma unroll
-                    for (int d = 0; d < ND; ++d) {
-                        const short4v v4 = *reinterpret_cast<const short4v*>(&vt[v_at<D>(key, d * 16 + 4 * fg)]);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (w != 0.f) o[d][qs][r] += w * (float)__builtin_bit_cast(T, (short)v4[r]);
-                    }
-                }
-            }
-        } else {
+        const short* const vt = ldsV;
+        {
             typedef short4v __attribute__((address_space(3)))* lds4;
             if constexpr (NK == 1) {
                 short4v pf[QT];
@@ -412,8 +395,6 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeAttnParams p, int
                     }
             }
         }
-        if (it + 1 < n_tiles) store_tile(buf ^ 1, it + 1);
-        __syncthreads();
     }
 
     // ---- join the waves that split the keys, then normalise and store, or leave the partial result to the second launch
@@ -425,6 +406,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeAttnParams p, int
             for (int d = 0; d < ND; ++d) { o[d][qs][0] *= vref; o[d][qs][1] *= vref; o[d][qs][2] *= vref; o[d][qs][3] *= vref; }
     }
     if constexpr (WK > 1) {
+        __syncthreads();                                     // the tile's memory is free
         if (fg == 0)
 #pragma unroll
             for (int qs = 0; qs < QT; ++qs) { red_m[wave][qs * 16 + fr] = m[qs]; red_l[wave][qs * 16 + fr] = l[qs]; }
@@ -469,6 +451,28 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeAttnParams p, int
     }
     constexpr int DW = ND / WK;
     const int d0 = WK > 1 ? wk * DW : 0;
+    if constexpr (WK == 1) __syncthreads();
+    if (bad_v) {                                             // (written before the last barrier)
+        for (int key = max(key0, kept); key < key1; ++key) {
+            const int pgid = pages[key >> p.c.page_shift];
+            if (pgid < 0 || pgid >= p.c.n_pages) continue;
+            const long at = (long)pgid * p.c.page_stride + g * p.c.head_stride + (long)(key & page_mask) * p.c.token_stride;
+#pragma unroll
+            for (int qs = 0; qs < QT; ++qs) {
+                if (!(visible(node[qs], key - kept) & 1)) continue;
+#pragma unroll
+                for (int d = 0; d < DW; ++d)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const long e = at + (d0 + d) * 16 + 4 * fg + r;
+                        float x;
+                        if constexpr (KV8) x = (static_cast<const uint8_t*>(p.c.v)[e] & 0x7f) == 0x7f ? __uint_as_float(0x7fc00000u) : 0.f;
+                        else x = (float)static_cast<const T*>(p.c.v)[e];
+                        if (!(fabsf(x) < INFINITY)) o[d][qs][r] += x;
+                    }
+            }
+        }
+    }
 #pragma unroll
     for (int qs = 0; qs < QT; ++qs) {
         const int c = cb * CB + (wq * QT + qs) * 16 + fr;
