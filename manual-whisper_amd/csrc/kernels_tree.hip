@@ -28,6 +28,7 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int KT = 64;                                       // keys of a tile
+constexpr float kGap = 6.f;
 
 template <typename T> struct Mat;
 template <> struct Mat<f16> {
@@ -69,14 +70,10 @@ __device__ __forceinline__ float column_sum(float v) {
     v += __shfl_xor(v, 16);
     return v + __shfl_xor(v, 32);
 }
-// LDS images of a tile: rows of D values in chunks of 8; the chunk index is exchanged by the row so that the rows that one
-// instruction reads (16 of K, 8 of V) start in different banks.
-template <int D> __device__ __forceinline__ int k_at(int row, int chunk) {
-    return row * D + ((chunk ^ (D == 64 ? (row >> 1) & 7 : row & 15)) << 3);
-}
-template <int D> __device__ __forceinline__ int v_at(int row, int col) {
-    return row * D + ((((col >> 3) ^ (D == 64 ? ((row >> 1) & 3) << 1 : (row & 7) << 1)) << 3) | (col & 7));
-}
+// LDS images of a tile: rows of K are D + 8 values apart, rows of V D + 16, so that the rows that one instruction reads (16
+// pieces of 16 bytes of K, 8 of 32 bytes of V) start in different banks and every address is one register and a constant.
+template <int D> __device__ __forceinline__ int k_at(int row, int chunk) { return row * (D + 8) + chunk * 8; }
+template <int D> __device__ __forceinline__ int v_at(int row, int col) { return row * (D + 16) + col; }
 // 8 e4m3 codes -> 8 values of T (exact)
 template <typename T> __device__ __forceinline__ short8v widen8(unsigned a, unsigned b) {
     typedef float f2 __attribute__((ext_vector_type(2)));
@@ -86,125 +83,127 @@ template <typename T> __device__ __forceinline__ short8v widen8(unsigned a, unsi
                    bits_of<T>(x2[0]), bits_of<T>(x2[1]), bits_of<T>(x3[0]), bits_of<T>(x3[1])};
 }
 
+// LDS of a workgroup: K and V of a tile (at the end: partial results of waves that split the keys), K's and V's row scales.
+template <bool KV8, int D> struct Shared {
+    short tiles[KT * (2 * D + 24)] __attribute__((aligned(16)));
+    float scales[2][KV8 ? KT : 4] __attribute__((aligned(16)));
+    int page_ok[4] __attribute__((aligned(16)));             // per 16 keys: the page exists
+    int bad_v;                                               // V rows of this step held an infinity or a NaN
+    float red_m[4][32], red_l[4][32];
+};
+// What a workgroup works on: keys key0 .. key1 of request b for K/V head g, query columns col0 .. of `cols`
+struct Work { int b, unit, pieces, g, row0, nodes, cols, col0, kept, key0, key1; };
+
 // T: type of q, of the products and of out.  KV8: the cache holds e4m3 codes with a scale per row; the codes go to the matrix
 // cores as they are, K's scale multiplies the score and V's the weight.  QT: 16-column query tiles per wave.  WK: waves that
 // share the columns and split a tile's keys; 4 / WK groups of waves hold different columns.
 template <typename T, bool KV8, int D, int QT, int WK>
-__global__ __launch_bounds__(256, QT == 1 ? (D == 64 ? 4 : 3) : 2) void tree_attn_kernel(TreeAttnParams p, int n_blocks, int group) {
-    constexpr int WQ = 4 / WK, NK = 4 / WK, CB = 16 * QT * WQ;
+__device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const Work& w, Shared<KV8, D>& lds) {
+    constexpr int NK = 4 / WK;                               // 16-key tiles of a wave
     constexpr int EPL = KV8 ? 16 : 8;                        // values of a 16-byte load
     constexpr int CPR = D / EPL, RPP = 256 / CPR, NI = KT / RPP;
     constexpr int ND = D / 16;
-    // K and V of a tile; at the end the partial results of the waves that split the keys
-    constexpr int kTile = 2 * KT * D, kJoin = WK > 1 ? 2 * 4 * 16 * QT * D : 0;
-    __shared__ __attribute__((aligned(16))) short tiles[kTile > kJoin ? kTile : kJoin];
-    __shared__ __attribute__((aligned(16))) float scales[2][KV8 ? KT : 4];
-    __shared__ __attribute__((aligned(16))) int page_ok[4];  // per 16 keys: the page exists
-    __shared__ int bad_v;                                    // V rows of this step held an infinity or a NaN
-    __shared__ float red_m[4][16 * QT], red_l[4][16 * QT];
-    short* const ldsK = tiles;
-    short* const ldsV = tiles + KT * D;
-
-    // workgroup -> (unit, K/V head, column block): the blocks of one (unit, head) are 8 ids apart, on the same XCD, so that
-    // its K/V rows come from that XCD's L2 after the first of them
-    const int pair = blockIdx.x / (8 * n_blocks) * 8 + (blockIdx.x & 7), cb = (blockIdx.x >> 3) % n_blocks;
-    const int unit = pair / p.c.heads, g = pair - unit * p.c.heads;
-    if (unit >= p.n_units) return;
-    const int4 work = reinterpret_cast<const int4*>(p.units)[unit];
-    const int b = work.x;
-    if (b < 0 || b >= p.batch) return;
-    const int row0 = max(0, p.row_start[b]);
-    const int nodes = min(min(p.row_start[b + 1], p.rows) - row0, p.max_nodes);
-    const int cols = nodes * group;
-    if (cb * CB >= cols) return;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    short* const ldsK = lds.tiles;
+    short* const ldsV = lds.tiles + KT * (D + 8);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int fr = lane & 15, fg = lane >> 4;
     const int wq = wave / WK, wk = wave % WK;
-    const int kept = max(0, p.kept[b]);
-    // keys of this workgroup: the unit's, none behind the last one that a row of this block can see
-    const int last_node = p.mask ? nodes - 1 : min(nodes - 1, (cb * CB + CB - 1) / group);
-    const int longest = p.max_pages << p.c.page_shift;
-    const int key0 = max(0, work.y) & ~(KT - 1);
-    const int key1 = (int)min((long)min(work.z, longest), (long)kept + last_node + 1);
+    const int key0 = w.key0, key1 = w.key1, kept = w.kept;
     const int n_tiles = key1 > key0 ? (key1 - key0 + KT - 1) / KT : 0;
+    const bool active = w.col0 + wq * QT * 16 < w.cols;      // wave-uniform; a wave without columns only helps with the staging
 
     // ---- the query columns of this wave
     short8v qf[QT][D / 32];
     int node[QT];
 #pragma unroll
     for (int qs = 0; qs < QT; ++qs) {
-        const int c = min(cb * CB + (wq * QT + qs) * 16 + fr, cols - 1);
+        const int c = min(w.col0 + (wq * QT + qs) * 16 + fr, w.cols - 1);
         node[qs] = c / group;
-        const short* src = static_cast<const short*>(p.q) + (long)(row0 + node[qs]) * p.q_row + (long)(g * group + c - node[qs] * group) * p.q_head;
+        const short* src = static_cast<const short*>(p.q) + (long)(w.row0 + node[qs]) * p.q_row + (long)(w.g * group + c - node[qs] * group) * p.q_head;
 #pragma unroll
         for (int s = 0; s < D / 32; ++s) qf[qs][s] = *reinterpret_cast<const short8v*>(src + s * 32 + fg * 8);
     }
+    const float to_log2 = p.scale * kLog2e;                  // exponents of two: weight = exp2((s - max) * scale * log2 e)
+    const float by = KV8 ? 1.f : to_log2;                    // what is left to multiply a score by
 
-    // ---- staging
+    // ---- staging.  The rows that a wave loads at once lie in one aligned run of 16 keys, so in one page: the page's address is
+    // scalar, and a lane adds an offset that is the same for every tile.
     const int ch = tid % CPR, srow = tid / CPR;
-    const int* const pages = p.table + (long)b * p.table_stride;
+    const int* const pages = p.table + (long)w.b * p.table_stride;
     const int page_mask = (1 << p.c.page_shift) - 1;
+    const int run = (wave * (64 / CPR)) >> 4;                // run of 16 keys within the first RPP rows
+    const int lane_off = (srow & 15) * (int)p.c.token_stride + ch * EPL;
     u32x4 rk[NI], rv[NI];
-    int pg[NI], pg_s = 0;                                    // pages of the rows to be loaded next
-    unsigned ok = 0;                                         // bit i: row i of the loaded tile exists
+    int pg[NI], pg_s = -1;                                   // pages of the rows to be loaded next
+    unsigned ok = 0;                                         // bit i: the page of rows i of the loaded tile exists
     float rscale = 0.f;
-    auto page_id = [&](int key) -> int { return key < key1 ? pages[key >> p.c.page_shift] : -1; };
+    bool ok_s = false;
+    // What is loaded here and in load_tile is looked at one tile later: a comparison here would wait for every load in flight.
+    auto page_id = [&](int key) -> int { return pages[min(key, key1 - 1) >> p.c.page_shift]; };
     auto load_pages = [&](int kv0) {
 #pragma unroll
-        for (int i = 0; i < NI; ++i) pg[i] = page_id(kv0 + srow + RPP * i);
+        for (int i = 0; i < NI; ++i) pg[i] = page_id(kv0 + 16 * run + RPP * i);
         if constexpr (KV8) pg_s = page_id(kv0 + (tid & (KT - 1)));
     };
     auto load_tile = [&](int kv0) {
         ok = 0;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const int key = kv0 + srow + RPP * i;
-            const bool there = pg[i] >= 0 && pg[i] < p.c.n_pages;
+            const int id = __builtin_amdgcn_readfirstlane(pg[i]);
+            const bool there = id >= 0 && id < p.c.n_pages;
             ok |= there ? 1u << i : 0u;
-            const long off = (long)(there ? pg[i] : 0) * p.c.page_stride + g * p.c.head_stride + (long)(key & page_mask) * p.c.token_stride + ch * EPL;
+            const long base = (long)(there ? id : 0) * p.c.page_stride + w.g * p.c.head_stride + (long)((kv0 + 16 * run + RPP * i) & page_mask) * p.c.token_stride;
+            // at most 16 columns: the rows are read once, and a step moves more than the caches hold
+            auto row16 = [&](const void* at) {
+                if constexpr (QT == 1) return __builtin_nontemporal_load(static_cast<const u32x4*>(at));
+                else return *static_cast<const u32x4*>(at);
+            };
             if constexpr (KV8) {
-                rk[i] = *reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(p.c.k) + off);
-                rv[i] = *reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(p.c.v) + off);
+                rk[i] = row16(static_cast<const uint8_t*>(p.c.k) + base + lane_off);
+                rv[i] = row16(static_cast<const uint8_t*>(p.c.v) + base + lane_off);
             } else {
-                rk[i] = *reinterpret_cast<const u32x4*>(static_cast<const short*>(p.c.k) + off);
-                rv[i] = *reinterpret_cast<const u32x4*>(static_cast<const short*>(p.c.v) + off);
+                rk[i] = row16(static_cast<const short*>(p.c.k) + base + lane_off);
+                rv[i] = row16(static_cast<const short*>(p.c.v) + base + lane_off);
             }
         }
         if constexpr (KV8) {
-            if (tid < 2 * KT) {
-                const bool there = pg_s >= 0 && pg_s < p.c.n_pages;
-                const long at = (((long)(there ? pg_s : 0) * p.c.heads + g) << p.c.page_shift) + ((kv0 + (tid & (KT - 1))) & page_mask);
-                rscale = there ? (tid < KT ? p.c.ks : p.c.vs)[at] : 0.f;
-            }
+            ok_s = pg_s >= 0 && pg_s < p.c.n_pages && kv0 + (tid & (KT - 1)) < key1;
+            const long at = (((long)(ok_s ? pg_s : 0) * p.c.heads + w.g) << p.c.page_shift) + ((kv0 + (tid & (KT - 1))) & page_mask);
+            rscale = (tid < KT ? p.c.ks : p.c.vs)[at];       // (the upper half of the workgroup's is not used)
         }
     };
     auto store_tile = [&](int it) {
-        // In tiles with rows of this step V's infinities and NaN are held back: in the product they would reach rows that do not
-        // see them (0 times NaN is NaN).  The rows that do get them at the end.
-        const bool own_step = key0 + it * KT + KT > kept;
+        const int kv0 = key0 + it * KT;
         bool bad = false;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int row = srow + RPP * i;
-            const bool there = ok >> i & 1;
-            const u32x4 none = {0, 0, 0, 0};
-            const u32x4 v = there ? rv[i] : none;            // what lies behind the last key may be anything
             if constexpr (KV8) {
                 *reinterpret_cast<short8v*>(&ldsK[k_at<D>(row, 2 * ch)]) = widen8<T>(rk[i][0], rk[i][1]);
                 *reinterpret_cast<short8v*>(&ldsK[k_at<D>(row, 2 * ch + 1)]) = widen8<T>(rk[i][2], rk[i][3]);
-                u32x4 lo = __builtin_bit_cast(u32x4, widen8<T>(v[0], v[1])), hi = __builtin_bit_cast(u32x4, widen8<T>(v[2], v[3]));
-                if (own_step) { lo = finite_only<T>(lo, bad); hi = finite_only<T>(hi, bad); }
-                *reinterpret_cast<u32x4*>(&ldsV[v_at<D>(row, 16 * ch)]) = lo;
-                *reinterpret_cast<u32x4*>(&ldsV[v_at<D>(row, 16 * ch + 8)]) = hi;
             } else {
                 *reinterpret_cast<u32x4*>(&ldsK[k_at<D>(row, ch)]) = rk[i];
-                *reinterpret_cast<u32x4*>(&ldsV[v_at<D>(row, 8 * ch)]) = own_step ? finite_only<T>(v, bad) : v;
             }
-            if (ch == 0 && (row & 15) == 0) page_ok[row >> 4] = there;
+            u32x4 lo = rv[i], hi = rv[i];
+            if constexpr (KV8) {
+                lo = __builtin_bit_cast(u32x4, widen8<T>(rv[i][0], rv[i][1]));
+                hi = __builtin_bit_cast(u32x4, widen8<T>(rv[i][2], rv[i][3]));
+            }
+            if (kv0 + KT > kept || !(ok >> i & 1)) {         // (uniform) tiles with rows of this step, or behind the last key
+                // V's infinities and NaN are held back here: in the product they would reach rows that do not see them (0 times
+                // NaN is NaN).  The rows that do get them at the end.  What lies behind the last key may be anything.
+                const u32x4 none = {0, 0, 0, 0};
+                if (kv0 + row >= key1 || !(ok >> i & 1)) lo = hi = none;
+                lo = finite_only<T>(lo, bad);
+                if constexpr (KV8) hi = finite_only<T>(hi, bad);
+            }
+            *reinterpret_cast<u32x4*>(&ldsV[v_at<D>(row, EPL * ch)]) = lo;
+            if constexpr (KV8) *reinterpret_cast<u32x4*>(&ldsV[v_at<D>(row, EPL * ch + 8)]) = hi;
+            if (ch == 0 && (row & 15) == 0) lds.page_ok[row >> 4] = ok >> i & 1;
         }
-        if (bad) bad_v = 1;
+        if (bad) lds.bad_v = 1;
         if constexpr (KV8) {
-            if (tid < 2 * KT) scales[tid / KT][tid & (KT - 1)] = rscale;
+            if (tid < 2 * KT) lds.scales[tid / KT][tid & (KT - 1)] = !ok_s ? 0.f : tid < KT ? rscale * to_log2 : rscale;
         }
     };
 
@@ -219,8 +218,6 @@ __global__ __launch_bounds__(256, QT == 1 ? (D == 64 ? 4 : 3) : 2) void tree_att
     // e4m3: weights are p_j times V's row scale relative to a power of two above every scale seen so far, so that they stay
     // within fp16's range whatever the scales are; the accumulators are multiplied by it at the end
     float vref = 0.f;
-    const float to_log2 = p.scale * kLog2e;
-
     // which of the 64 keys from node `first` on (negative: kept tokens before it) the row of node `n` sees
     auto visible = [&](int n, int first) -> unsigned long long {
         if (first <= -64) return ~0ull;
@@ -228,14 +225,14 @@ __global__ __launch_bounds__(256, QT == 1 ? (D == 64 ? 4 : 3) : 2) void tree_att
             const int c = n - first + 1;
             return c <= 0 ? 0ull : c >= 64 ? ~0ull : (1ull << c) - 1;
         }
-        const unsigned* words = p.mask + (long)(row0 + n) * p.mask_words;
-        auto word = [&](int w) -> unsigned long long { return w < p.mask_words ? words[w] : 0u; };
+        const unsigned* words = p.mask + (long)(w.row0 + n) * p.mask_words;
+        auto word = [&](int i) -> unsigned long long { return i < p.mask_words ? words[i] : 0u; };
         if (first < 0) return ((word(0) | word(1) << 32) << -first) | ((1ull << -first) - 1);
-        const int w = first >> 5, sh = first & 31;
-        const unsigned long long x = (word(w) | word(w + 1) << 32) >> sh;
-        return sh ? x | word(w + 2) << (64 - sh) : x;
+        const int i = first >> 5, sh = first & 31;
+        const unsigned long long x = (word(i) | word(i + 1) << 32) >> sh;
+        return sh ? x | word(i + 2) << (64 - sh) : x;
     };
-    if (tid == 0) bad_v = 0;
+    if (tid == 0) lds.bad_v = 0;
     if (n_tiles > 0) {
         load_pages(key0);
         load_tile(key0);
@@ -250,6 +247,8 @@ __global__ __launch_bounds__(256, QT == 1 ? (D == 64 ? 4 : 3) : 2) void tree_att
             load_tile(kv0 + KT);
             load_pages(kv0 + 2 * KT);
         }
+        __builtin_amdgcn_sched_barrier(0);                   // phases stay apart: mixed, their operands do not fit the registers
+        if (!active) continue;
         // ---- S^T
         float4v sc[NK][QT];
 #pragma unroll
@@ -264,20 +263,19 @@ __global__ __launch_bounds__(256, QT == 1 ? (D == 64 ? 4 : 3) : 2) void tree_att
                 for (int qs = 0; qs < QT; ++qs) sc[i][qs] = Mat<T>::mma32(kf, qf[qs][s], sc[i][qs]);
             }
         }
-        // ---- scores in units of log2; the keys that a column does not see
-        const int4 there = *reinterpret_cast<const int4*>(page_ok);
+        __builtin_amdgcn_sched_barrier(0);
+        // ---- the keys that a column does not see
+        const int4 there = *reinterpret_cast<const int4*>(lds.page_ok);
         const bool edge = kv0 + KT > kept || kv0 + KT > key1 || !(there.x && there.y && there.z && there.w);
+        if constexpr (KV8) {                                 // K's row scales (already times scale * log2 e)
 #pragma unroll
-        for (int i = 0; i < NK; ++i) {
-            float4v by = float4v{to_log2, to_log2, to_log2, to_log2};
-            if constexpr (KV8) {
-                const float4v s4 = *reinterpret_cast<const float4v*>(&scales[0][(wk * NK + i) * 16 + 4 * fg]);
-                by = float4v{s4[0] * to_log2, s4[1] * to_log2, s4[2] * to_log2, s4[3] * to_log2};
+            for (int i = 0; i < NK; ++i) {
+                const float4v s4 = *reinterpret_cast<const float4v*>(&lds.scales[0][(wk * NK + i) * 16 + 4 * fg]);
+#pragma unroll
+                for (int qs = 0; qs < QT; ++qs)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) sc[i][qs][r] *= s4[r];
             }
-#pragma unroll
-            for (int qs = 0; qs < QT; ++qs)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) sc[i][qs][r] *= by[r];
         }
         if (edge) {
             const int first = kv0 - kept, limit = key1 - kv0;                 // node of the tile's first key (may be negative)
@@ -296,47 +294,44 @@ __global__ __launch_bounds__(256, QT == 1 ? (D == 64 ? 4 : 3) : 2) void tree_att
                         if (!(sees >> ((wk * NK + i) * 16 + 4 * fg + r) & 1)) sc[i][qs][r] = -INFINITY;
             }
         }
-        // ---- online softmax
-        float mn[QT];
+        // ---- online softmax.  m is the reference of a column's weights, 2^(s - m): it rises only when a score exceeds it by more
+        // than kGap, so that weights stay below 2^kGap and the lanes of a column need not agree on a maximum in every tile.
         bool lift = false;
+        float top[QT];
 #pragma unroll
         for (int qs = 0; qs < QT; ++qs) {
-            float x = -INFINITY;
+            top[qs] = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < NK; ++i) x = fmaxf(x, fmaxf(fmaxf(sc[i][qs][0], sc[i][qs][1]), fmaxf(sc[i][qs][2], sc[i][qs][3])));
-            mn[qs] = fmaxf(m[qs], column_max(x));
-            lift = lift || mn[qs] > m[qs];
+            for (int i = 0; i < NK; ++i) top[qs] = fmaxf(top[qs], fmaxf(fmaxf(sc[i][qs][0], sc[i][qs][1]), fmaxf(sc[i][qs][2], sc[i][qs][3])));
+            lift = lift || top[qs] * by > m[qs] + kGap;
         }
-        if (__any(lift)) {
-#pragma unroll
-            for (int qs = 0; qs < QT; ++qs) {
-                const float alpha = mn[qs] > m[qs] ? __builtin_amdgcn_exp2f(m[qs] - mn[qs]) : 1.f;
-                m[qs] = mn[qs];
-                l[qs] *= alpha;
-#pragma unroll
-                for (int d = 0; d < ND; ++d) { o[d][qs][0] *= alpha; o[d][qs][1] *= alpha; o[d][qs][2] *= alpha; o[d][qs][3] *= alpha; }
-            }
-        }
-        float vinv = 0.f;
+        float big = 0.f;                                     // e4m3: V's largest row scale in this tile, the same in all lanes
         if constexpr (KV8) {
-            float top = 0.f;
 #pragma unroll
             for (int i = 0; i < NK; ++i) {
-                const float4v s4 = *reinterpret_cast<const float4v*>(&scales[1][(wk * NK + i) * 16 + 4 * fg]);
-                top = fmaxf(top, fmaxf(fmaxf(s4[0], s4[1]), fmaxf(s4[2], s4[3])));
+                const float4v s4 = *reinterpret_cast<const float4v*>(&lds.scales[1][(wk * NK + i) * 16 + 4 * fg]);
+                big = fmaxf(big, fmaxf(fmaxf(s4[0], s4[1]), fmaxf(s4[2], s4[3])));
             }
-            top = column_max(top);
-            if (top > vref) {                                // the same in all lanes
-                const float up = __uint_as_float(min((__float_as_uint(top) & 0x7f800000u) + 0x00800000u, 0x7f000000u));
-                const float f = vref / up;
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-#pragma unroll
-                    for (int qs = 0; qs < QT; ++qs) { o[d][qs][0] *= f; o[d][qs][1] *= f; o[d][qs][2] *= f; o[d][qs][3] *= f; }
+            big = column_max(big);
+        }
+        if (__any(lift) || big > vref) {                     // wave-uniform
+            float f = 1.f;
+            if (KV8 && big > vref) {
+                const float up = __uint_as_float(min((__float_as_uint(big) & 0x7f800000u) + 0x00800000u, 0x7f000000u));
+                f = vref / up;
                 vref = up;
             }
-            vinv = vref > 0.f ? 1.f / vref : 0.f;
+#pragma unroll
+            for (int qs = 0; qs < QT; ++qs) {
+                const float mn = fmaxf(m[qs], column_max(top[qs]) * by);
+                const float alpha = mn > m[qs] ? __builtin_amdgcn_exp2f(m[qs] - mn) : 1.f;
+                m[qs] = mn;
+                l[qs] *= alpha;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) { o[d][qs][0] *= alpha * f; o[d][qs][1] *= alpha * f; o[d][qs][2] *= alpha * f; o[d][qs][3] *= alpha * f; }
+            }
         }
+        const float vinv = KV8 && vref > 0.f ? 1.f / vref : 0.f;
 #pragma unroll
         for (int qs = 0; qs < QT; ++qs) {
             const float ref = m[qs] == -INFINITY ? 0.f : m[qs];               // nothing seen yet: every weight is 0
@@ -344,17 +339,18 @@ __global__ __launch_bounds__(256, QT == 1 ? (D == 64 ? 4 : 3) : 2) void tree_att
 #pragma unroll
             for (int i = 0; i < NK; ++i) {
                 float4v vs4 = float4v{1, 1, 1, 1};
-                if constexpr (KV8) vs4 = *reinterpret_cast<const float4v*>(&scales[1][(wk * NK + i) * 16 + 4 * fg]);
+                if constexpr (KV8) vs4 = *reinterpret_cast<const float4v*>(&lds.scales[1][(wk * NK + i) * 16 + 4 * fg]);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float w = __builtin_amdgcn_exp2f(sc[i][qs][r] - ref);
-                    sum += w;
-                    if constexpr (KV8) sc[i][qs][r] = edge && w == 0.f ? 0.f : w * (vs4[r] * vinv);
-                    else sc[i][qs][r] = w;
+                    const float e = __builtin_amdgcn_exp2f(KV8 ? sc[i][qs][r] - ref : fmaf(sc[i][qs][r], to_log2, -ref));
+                    sum += e;
+                    if constexpr (KV8) sc[i][qs][r] = edge && e == 0.f ? 0.f : e * (vs4[r] * vinv);
+                    else sc[i][qs][r] = e;
                 }
             }
             l[qs] += sum;                                    // of this lane's keys; the column's sum is formed at the end
         }
+        __builtin_amdgcn_sched_barrier(0);
         // ---- O^T += V^T P^T.  The weights are rounded once to T (half a step of T each, as the result is); the sum above is of
         // the unrounded ones.
         const short* const vt = ldsV;
@@ -405,58 +401,50 @@ __global__ __launch_bounds__(256, QT == 1 ? (D == 64 ? 4 : 3) : 2) void tree_att
 #pragma unroll
             for (int d = 0; d < ND; ++d) { o[d][qs][0] *= vref; o[d][qs][1] *= vref; o[d][qs][2] *= vref; o[d][qs][3] *= vref; }
     }
+    constexpr int DW = ND / WK;                              // 16-dim tiles of the result that a wave ends up with
+    const int d0 = WK > 1 ? wk * DW : 0;
     if constexpr (WK > 1) {
-        __syncthreads();                                     // the tile's memory is free
         if (fg == 0)
 #pragma unroll
-            for (int qs = 0; qs < QT; ++qs) { red_m[wave][qs * 16 + fr] = m[qs]; red_l[wave][qs * 16 + fr] = l[qs]; }
-        __syncthreads();
+            for (int qs = 0; qs < QT; ++qs) { lds.red_m[wave][qs * 16 + fr] = m[qs]; lds.red_l[wave][qs * 16 + fr] = l[qs]; }
+        float* const ex = reinterpret_cast<float*>(lds.tiles);
 #pragma unroll
         for (int qs = 0; qs < QT; ++qs) {
+            __syncthreads();                                 // the tile's memory is free; all maxima are there
             float all = -INFINITY, sum = 0.f;
 #pragma unroll
-            for (int w = 0; w < WK; ++w) all = fmaxf(all, red_m[wq * WK + w][qs * 16 + fr]);
+            for (int k = 0; k < WK; ++k) all = fmaxf(all, lds.red_m[wq * WK + k][qs * 16 + fr]);
             const float ref = all == -INFINITY ? 0.f : all;
 #pragma unroll
-            for (int w = 0; w < WK; ++w) sum += red_l[wq * WK + w][qs * 16 + fr] * __builtin_amdgcn_exp2f(red_m[wq * WK + w][qs * 16 + fr] - ref);
+            for (int k = 0; k < WK; ++k) sum += lds.red_l[wq * WK + k][qs * 16 + fr] * __builtin_amdgcn_exp2f(lds.red_m[wq * WK + k][qs * 16 + fr] - ref);
             const float f = __builtin_amdgcn_exp2f(m[qs] - ref);
             m[qs] = all; l[qs] = sum;
-#pragma unroll
-            for (int d = 0; d < ND; ++d) { o[d][qs][0] *= f; o[d][qs][1] *= f; o[d][qs][2] *= f; o[d][qs][3] *= f; }
-        }
-        // a wave's O as [columns][D] floats; wave w of the group adds up the columns' dims [w * D / WK, ...)
-        float* const ex = reinterpret_cast<float*>(tiles);
-        constexpr int WCOLS = 16 * QT;
-#pragma unroll
-        for (int qs = 0; qs < QT; ++qs)
+            // a wave's O as [16 columns][D] floats, chunks of four exchanged by the column; then wave k of the group adds up
+            // the head dims [k D / WK, ...) of all of its waves, in wave order
 #pragma unroll
             for (int d = 0; d < ND; ++d)
-                *reinterpret_cast<float4v*>(&ex[((wave * WCOLS) + qs * 16 + fr) * D + (((d * 4 + fg) ^ fr) & (D / 4 - 1)) * 4]) = o[d][qs];
-        __syncthreads();
-        constexpr int DW = ND / WK;                          // 16-dim tiles that a wave adds up
-#pragma unroll
-        for (int qs = 0; qs < QT; ++qs)
+                *reinterpret_cast<float4v*>(&ex[(wave * 16 + fr) * D + ((d * 4 + fg) ^ fr) * 4]) =
+                    float4v{o[d][qs][0] * f, o[d][qs][1] * f, o[d][qs][2] * f, o[d][qs][3] * f};
+            __syncthreads();
 #pragma unroll
             for (int d = 0; d < DW; ++d) {
-                float4v t = float4v{0, 0, 0, 0};
+                float4v sum4 = float4v{0, 0, 0, 0};
 #pragma unroll
-                for (int w = 0; w < WK; ++w) {
-                    const float4v x = *reinterpret_cast<const float4v*>(
-                        &ex[(((wq * WK + w) * WCOLS) + qs * 16 + fr) * D + ((((wk * DW + d) * 4 + fg) ^ fr) & (D / 4 - 1)) * 4]);
+                for (int k = 0; k < WK; ++k) {
+                    const float4v x = *reinterpret_cast<const float4v*>(&ex[((wq * WK + k) * 16 + fr) * D + (((d0 + d) * 4 + fg) ^ fr) * 4]);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) t[r] += x[r];
+                    for (int r = 0; r < 4; ++r) sum4[r] += x[r];
                 }
-                o[d][qs] = t;
+                o[d][qs] = sum4;
             }
+        }
     }
-    constexpr int DW = ND / WK;
-    const int d0 = WK > 1 ? wk * DW : 0;
     if constexpr (WK == 1) __syncthreads();
-    if (bad_v) {                                             // (written before the last barrier)
+    if (lds.bad_v) {                                         // (written before the last barrier)
         for (int key = max(key0, kept); key < key1; ++key) {
             const int pgid = pages[key >> p.c.page_shift];
             if (pgid < 0 || pgid >= p.c.n_pages) continue;
-            const long at = (long)pgid * p.c.page_stride + g * p.c.head_stride + (long)(key & page_mask) * p.c.token_stride;
+            const long at = (long)pgid * p.c.page_stride + w.g * p.c.head_stride + (long)(key & page_mask) * p.c.token_stride;
 #pragma unroll
             for (int qs = 0; qs < QT; ++qs) {
                 if (!(visible(node[qs], key - kept) & 1)) continue;
@@ -475,17 +463,17 @@ __global__ __launch_bounds__(256, QT == 1 ? (D == 64 ? 4 : 3) : 2) void tree_att
     }
 #pragma unroll
     for (int qs = 0; qs < QT; ++qs) {
-        const int c = cb * CB + (wq * QT + qs) * 16 + fr;
-        if (c >= cols) continue;
-        if (work.w <= 1 || !p.workspace) {
+        const int c = w.col0 + (wq * QT + qs) * 16 + fr;
+        if (c >= w.cols) continue;
+        if (w.pieces <= 1 || !p.workspace) {
             const float inv = l[qs] == 0.f ? 0.f : 1.f / l[qs];               // (a NaN sum stays NaN)
-            short* dst = static_cast<short*>(p.out) + (long)(row0 + node[qs]) * p.out_row + (long)(g * group + c - node[qs] * group) * p.out_head;
+            short* dst = static_cast<short*>(p.out) + (long)(w.row0 + node[qs]) * p.out_row + (long)(w.g * group + c - node[qs] * group) * p.out_head;
 #pragma unroll
             for (int d = 0; d < DW; ++d)
                 *reinterpret_cast<short4v*>(dst + (d0 + d) * 16 + 4 * fg) =
                     short4v{bits_of<T>(o[d][qs][0] * inv), bits_of<T>(o[d][qs][1] * inv), bits_of<T>(o[d][qs][2] * inv), bits_of<T>(o[d][qs][3] * inv)};
         } else {
-            const long slot = ((long)unit * p.c.heads + g) * (p.max_nodes * group) + c;
+            const long slot = ((long)w.unit * p.c.heads + w.g) * (p.max_nodes * group) + c;
             float* po = p.workspace + slot * D;
 #pragma unroll
             for (int d = 0; d < DW; ++d) *reinterpret_cast<float4v*>(po + (d0 + d) * 16 + 4 * fg) = o[d][qs];
@@ -497,51 +485,109 @@ __global__ __launch_bounds__(256, QT == 1 ? (D == 64 ? 4 : 3) : 2) void tree_att
     }
 }
 
-// Rows of requests that were cut: the units' partial results, weighted by their maxima.  One workgroup per (request, node).
+// Workgroup -> (unit, K/V head, column block): the blocks of one (unit, head) are 8 ids apart, on the same XCD, so that its K/V
+// rows come from that XCD's L2 after the first of them.  False: nothing to do.
+__device__ __forceinline__ bool find_work(const TreeAttnParams& p, int n_blocks, int group, int block, Work& w) {
+    const int pair = blockIdx.x / (8 * n_blocks) * 8 + (blockIdx.x & 7), cb = (blockIdx.x >> 3) % n_blocks;
+    w.unit = pair / p.c.heads; w.g = pair - w.unit * p.c.heads;
+    if (w.unit >= p.n_units) return false;
+    const int4 u = reinterpret_cast<const int4*>(p.units)[w.unit];
+    w.b = u.x; w.pieces = u.w;
+    if (w.b < 0 || w.b >= p.batch) return false;
+    w.row0 = max(0, p.row_start[w.b]);
+    w.nodes = min(min(p.row_start[w.b + 1], p.rows) - w.row0, p.max_nodes);
+    w.cols = w.nodes * group;
+    w.col0 = cb * block;
+    if (w.col0 >= w.cols) return false;
+    w.kept = max(0, p.kept[w.b]);
+    // keys: the unit's, none behind the last one that a row of this block can see
+    const int last_node = p.mask ? w.nodes - 1 : min(w.nodes - 1, (w.col0 + block - 1) / group);
+    w.key0 = max(0, u.y) & ~(KT - 1);
+    w.key1 = (int)min((long)min(u.z, p.max_pages << p.c.page_shift), (long)w.kept + last_node + 1);
+    return true;
+}
+// At most 16 columns: a stream of K/V through the compute units; registers are held down for more workgroups on each.
+template <typename T, bool KV8, int D>
+__global__ __launch_bounds__(256, D == 64 ? 4 : 3) void tree_attn_narrow_kernel(TreeAttnParams p, int n_blocks, int group) {
+    __shared__ Shared<KV8, D> lds;
+    Work w;
+    if (find_work(p, n_blocks, group, 16, w)) attend<T, KV8, D, 1, 4>(p, group, w, lds);
+}
+// Up to 128 columns a workgroup; how the four waves share columns and keys goes by the columns that this request has left.
+template <typename T, bool KV8, int D>
+__global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeAttnParams p, int n_blocks, int group) {
+    __shared__ Shared<KV8, D> lds;
+    Work w;
+    if (!find_work(p, n_blocks, group, 128, w)) return;
+    const int left = w.cols - w.col0;
+    if (left <= 32) attend<T, KV8, D, 2, 4>(p, group, w, lds);
+    else if (left <= 64) attend<T, KV8, D, 2, 2>(p, group, w, lds);
+    else attend<T, KV8, D, 2, 1>(p, group, w, lds);
+}
+
+// Rows of requests that were cut: the units' partial results, weighted by their maxima.  One wave per (row, query head); its
+// groups of D / 4 lanes take the units in turn, eight loads ahead, and are joined by a butterfly.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeAttnParams p, int group) {
-    const int b = blockIdx.x / p.max_nodes, i = blockIdx.x - b * p.max_nodes;
+    constexpr int LANES = D / 4, GROUPS = 64 / LANES, AHEAD = 8;
+    const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const int h = (int)(id % p.heads);
+    const long bi = id / p.heads;
+    const int b = (int)(bi / p.max_nodes), i = (int)(bi - (long)b * p.max_nodes);
+    if (b >= p.batch) return;
     const int u0 = p.unit_start[b], n = p.unit_start[b + 1] - u0;
     const int row = p.row_start[b] + i;
     if (n < 2 || u0 < 0 || u0 + n > p.n_units || p.row_start[b] < 0 || row >= p.row_start[b + 1] || row >= p.rows) return;
-    const long cols = (long)p.max_nodes * group;
-    const float* const all_ml = p.workspace + (long)p.n_units * p.c.heads * cols * D;
-    for (int e = threadIdx.x; e < p.heads * (D / 4); e += 256) {
-        const int h = e / (D / 4), d = (e - h * (D / 4)) * 4;
-        const int g = h / group;
-        const long c = (long)i * group + (h - g * group);
-        float top = -INFINITY;
-        for (int u = 0; u < n; ++u) top = fmaxf(top, all_ml[(((long)(u0 + u) * p.c.heads + g) * cols + c) * 2]);
-        const float ref = top == -INFINITY ? 0.f : top;
-        float4v acc = float4v{0, 0, 0, 0};
-        float sum = 0.f;
-        for (int u = 0; u < n; ++u) {
-            const long slot = ((long)(u0 + u) * p.c.heads + g) * cols + c;
-            const float f = __builtin_amdgcn_exp2f(all_ml[slot * 2] - ref);
-            sum += f * all_ml[slot * 2 + 1];
-            const float4v x = *reinterpret_cast<const float4v*>(p.workspace + slot * D + d);
+    const int g = h / group, part = lane / LANES, d = (lane % LANES) * 4;
+    const long cols = (long)p.max_nodes * group, step = p.c.heads * cols;               // slots from one unit to the next
+    const long first = ((long)u0 * p.c.heads + g) * cols + (long)i * group + (h - g * group);
+    const float* const po = p.workspace;
+    const float* const ml = p.workspace + (long)p.n_units * step * D;
+    float m = -INFINITY, l = 0.f;
+    float4v acc = float4v{0, 0, 0, 0};
+    auto add = [&](float um, float ul, float4v x) {
+        const float mn = fmaxf(m, um), ref = mn == -INFINITY ? 0.f : mn;
+        const float fo = __builtin_amdgcn_exp2f(m - ref), fu = __builtin_amdgcn_exp2f(um - ref);
+        m = mn;
+        l = l * fo + ul * fu;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[r] += f * x[r];
+        for (int r = 0; r < 4; ++r) acc[r] = acc[r] * fo + x[r] * fu;
+    };
+    for (int u = part; u < n; u += GROUPS * AHEAD) {
+        float um[AHEAD], ul[AHEAD];
+        float4v x[AHEAD];
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            if (u + a * GROUPS >= n) continue;
+            const long slot = first + (u + a * GROUPS) * step;
+            um[a] = ml[slot * 2]; ul[a] = ml[slot * 2 + 1];
+            x[a] = *reinterpret_cast<const float4v*>(po + slot * D + d);
         }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        *reinterpret_cast<short4v*>(static_cast<short*>(p.out) + (long)row * p.out_row + (long)h * p.out_head + d) =
-            short4v{bits_of<T>(acc[0] * inv), bits_of<T>(acc[1] * inv), bits_of<T>(acc[2] * inv), bits_of<T>(acc[3] * inv)};
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a)
+            if (u + a * GROUPS < n) add(um[a], ul[a], x[a]);
     }
+#pragma unroll
+    for (int s = LANES; s < 64; s <<= 1)
+        add(__shfl_xor(m, s), __shfl_xor(l, s), float4v{__shfl_xor(acc[0], s), __shfl_xor(acc[1], s), __shfl_xor(acc[2], s), __shfl_xor(acc[3], s)});
+    if (part) return;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<short4v*>(static_cast<short*>(p.out) + (long)row * p.out_row + (long)h * p.out_head + d) =
+        short4v{bits_of<T>(acc[0] * inv), bits_of<T>(acc[1] * inv), bits_of<T>(acc[2] * inv), bits_of<T>(acc[3] * inv)};
 }
 
 template <typename T, bool KV8, int D>
 void launch_tree_t(const TreeAttnParams& p, hipStream_t s) {
     const int group = p.heads / p.c.heads;
     const long cols = (long)p.max_nodes * group;
-    const int block = cols <= 16 ? 16 : cols <= 32 ? 32 : cols <= 64 ? 64 : 128;
+    const int block = cols <= 16 ? 16 : 128;
     const int n_blocks = (int)((cols + block - 1) / block);
     const long pairs = ((long)p.n_units * p.c.heads + 7) / 8 * 8;
     const unsigned grid = (unsigned)(pairs * n_blocks);
-    if (block == 16) tree_attn_kernel<T, KV8, D, 1, 4><<<grid, 256, 0, s>>>(p, n_blocks, group);
-    else if (block == 32) tree_attn_kernel<T, KV8, D, 2, 4><<<grid, 256, 0, s>>>(p, n_blocks, group);
-    else if (block == 64) tree_attn_kernel<T, KV8, D, 2, 2><<<grid, 256, 0, s>>>(p, n_blocks, group);
-    else tree_attn_kernel<T, KV8, D, 2, 1><<<grid, 256, 0, s>>>(p, n_blocks, group);
-    if (p.n_units > p.batch) tree_join_kernel<T, D><<<(unsigned)((long)p.batch * p.max_nodes), 256, 0, s>>>(p, group);
+    if (block == 16) tree_attn_narrow_kernel<T, KV8, D><<<grid, 256, 0, s>>>(p, n_blocks, group);
+    else tree_attn_wide_kernel<T, KV8, D><<<grid, 256, 0, s>>>(p, n_blocks, group);
+    if (p.n_units > p.batch) tree_join_kernel<T, D><<<(unsigned)(((long)p.batch * p.max_nodes * p.heads + 3) / 4), 256, 0, s>>>(p, group);
 }
 
 }  // namespace

@@ -54,6 +54,7 @@ int check_cache(const char* who, const mw_paged_cache* c) {
     REFUSE_IF(c->page_stride % unit || c->head_stride % unit || c->token_stride % unit || misaligned(c->k, 16) || misaligned(c->v, 16),
               "rows of the cache must start at multiples of 16 bytes");
     REFUSE_IF(c->token_stride < c->head_dim || c->head_stride < c->head_dim || c->page_stride < c->head_dim, "strides of the cache must be at least head_dim");
+    REFUSE_IF(c->token_stride > (1 << 26), "token_stride must be at most 2^26");
     return MW_OK;
 }
 int log2i(int n) { int s = 0; while ((1 << s) < n) ++s; return s; }
@@ -151,7 +152,7 @@ extern "C" int mw_tree_attention(const mw_tree_args* a, int device, void* stream
     REFUSE_IF(need && (!a->workspace || a->workspace_bytes < need || misaligned(a->workspace, 16)),
               "the workspace is smaller than mw_tree_attention_workspace() or not 16-byte aligned");
     REFUSE_IF(((int64_t)a->n_units * a->cache.n_heads + 8) * (((int64_t)a->max_nodes * group + 127) / 128 + 1) >= INT32_MAX ||
-              (int64_t)a->batch * a->max_nodes >= INT32_MAX, "too many units or rows for one launch");
+              (int64_t)a->batch * a->max_nodes * a->n_heads >= INT32_MAX, "too many units or rows for one launch");
     OnDevice on(device);
     if (on.err != hipSuccess) return launched(who, on.err);
     TreeAttnParams p{};
