@@ -238,6 +238,11 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
         load_tile(key0);
         load_pages(key0 + KT);
     }
+    // the queries are here before the first product: a wait for them inside the loop would be one for all loads in flight
+#pragma unroll
+    for (int qs = 0; qs < QT; ++qs)
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) asm volatile("" : "+v"(qf[qs][s]));
     for (int it = 0; it < n_tiles; ++it) {
         const int kv0 = key0 + it * KT;
         __syncthreads();                                     // the previous tile has been read
@@ -525,13 +530,15 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeAttnParams p
     else attend<T, KV8, D, 2, 1>(p, group, w, lds);
 }
 
-// Rows of requests that were cut: the units' partial results, weighted by their maxima.  One wave per (row, query head); its
-// groups of D / 4 lanes take the units in turn, eight loads ahead, and are joined by a butterfly.
-template <typename T, int D>
+// Rows of requests that were cut: the units' partial results, weighted by their maxima.  WAVES waves per (row, query head); their
+// groups of D / 4 lanes take the units in turn, eight loads ahead, and are joined by a butterfly, waves through LDS.
+template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeAttnParams p, int group) {
     constexpr int LANES = D / 4, GROUPS = 64 / LANES, AHEAD = 8;
-    const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
+    __shared__ float red_m[WAVES], red_l[WAVES];
+    __shared__ __attribute__((aligned(16))) float red_o[WAVES][D];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const long id = WAVES == 1 ? (long)blockIdx.x * 4 + wave : blockIdx.x;
     const int h = (int)(id % p.heads);
     const long bi = id / p.heads;
     const int b = (int)(bi / p.max_nodes), i = (int)(bi - (long)b * p.max_nodes);
@@ -539,7 +546,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeAttnParams p, int gr
     const int u0 = p.unit_start[b], n = p.unit_start[b + 1] - u0;
     const int row = p.row_start[b] + i;
     if (n < 2 || u0 < 0 || u0 + n > p.n_units || p.row_start[b] < 0 || row >= p.row_start[b + 1] || row >= p.rows) return;
-    const int g = h / group, part = lane / LANES, d = (lane % LANES) * 4;
+    const int g = h / group, part = lane / LANES + (WAVES == 1 ? 0 : wave * GROUPS), d = (lane % LANES) * 4;
     const long cols = (long)p.max_nodes * group, step = p.c.heads * cols;               // slots from one unit to the next
     const long first = ((long)u0 * p.c.heads + g) * cols + (long)i * group + (h - g * group);
     const float* const po = p.workspace;
@@ -554,23 +561,30 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeAttnParams p, int gr
 #pragma unroll
         for (int r = 0; r < 4; ++r) acc[r] = acc[r] * fo + x[r] * fu;
     };
-    for (int u = part; u < n; u += GROUPS * AHEAD) {
+    for (int u = part; u < n; u += GROUPS * WAVES * AHEAD) {
         float um[AHEAD], ul[AHEAD];
         float4v x[AHEAD];
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a) {
-            if (u + a * GROUPS >= n) continue;
-            const long slot = first + (u + a * GROUPS) * step;
+            const long slot = first + min(u + a * GROUPS * WAVES, n - 1) * step;
             um[a] = ml[slot * 2]; ul[a] = ml[slot * 2 + 1];
             x[a] = *reinterpret_cast<const float4v*>(po + slot * D + d);
         }
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a)
-            if (u + a * GROUPS < n) add(um[a], ul[a], x[a]);
+            if (u + a * GROUPS * WAVES < n) add(um[a], ul[a], x[a]);
     }
 #pragma unroll
     for (int s = LANES; s < 64; s <<= 1)
         add(__shfl_xor(m, s), __shfl_xor(l, s), float4v{__shfl_xor(acc[0], s), __shfl_xor(acc[1], s), __shfl_xor(acc[2], s), __shfl_xor(acc[3], s)});
+    if constexpr (WAVES > 1) {
+        if (lane == 0) { red_m[wave] = m; red_l[wave] = l; }
+        if (lane < LANES) *reinterpret_cast<float4v*>(&red_o[wave][d]) = acc;
+        __syncthreads();
+        m = -INFINITY; l = 0.f; acc = float4v{0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < WAVES; ++k) add(red_m[k], red_l[k], *reinterpret_cast<const float4v*>(&red_o[k][d]));
+    }
     if (part) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     *reinterpret_cast<short4v*>(static_cast<short*>(p.out) + (long)row * p.out_row + (long)h * p.out_head + d) =
@@ -587,7 +601,13 @@ void launch_tree_t(const TreeAttnParams& p, hipStream_t s) {
     const unsigned grid = (unsigned)(pairs * n_blocks);
     if (block == 16) tree_attn_narrow_kernel<T, KV8, D><<<grid, 256, 0, s>>>(p, n_blocks, group);
     else tree_attn_wide_kernel<T, KV8, D><<<grid, 256, 0, s>>>(p, n_blocks, group);
-    if (p.n_units > p.batch) tree_join_kernel<T, D><<<(unsigned)(((long)p.batch * p.max_nodes * p.heads + 3) / 4), 256, 0, s>>>(p, group);
+    if (p.n_units > p.batch) {
+        // few rows have few waves: four of them share a row's units then (8 requests of 1 row, 32 heads, up to 80 units: 15.5 ->
+        // 5.5 us); for many rows one wave each is faster (32 trees, 8 units at most: 44 -> 29 us)
+        const long pairs = (long)p.batch * p.max_nodes * p.heads;
+        if (pairs <= 4096) tree_join_kernel<T, D, 4><<<(unsigned)pairs, 256, 0, s>>>(p, group);
+        else tree_join_kernel<T, D, 1><<<(unsigned)((pairs + 3) / 4), 256, 0, s>>>(p, group);
+    }
 }
 
 }  // namespace
