@@ -101,7 +101,7 @@ template <typename T, bool KV8, int D, int QT, int WK>
 __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const Work& w, Shared<KV8, D>& lds) {
     constexpr int NK = 4 / WK;                               // 16-key tiles of a wave
     constexpr int EPL = KV8 ? 16 : 8;                        // values of a 16-byte load
-    constexpr int CPR = D / EPL, RPP = 256 / CPR, NI = KT / RPP;
+    constexpr int CPR = D / EPL, RPL = 64 / CPR, NI = 16 / RPL;               // lanes of a row, rows of a load, loads of 16 rows
     constexpr int ND = D / 16;
     short* const ldsK = lds.tiles;
     short* const ldsV = lds.tiles + KT * (D + 8);
@@ -126,58 +126,47 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
     const float to_log2 = p.scale * kLog2e;                  // exponents of two: weight = exp2((s - max) * scale * log2 e)
     const float by = KV8 ? 1.f : to_log2;                    // what is left to multiply a score by
 
-    // ---- staging.  The rows that a wave loads at once lie in one aligned run of 16 keys, so in one page: the page's address is
-    // scalar, and a lane adds an offset that is the same for every tile.
-    const int ch = tid % CPR, srow = tid / CPR;
+    // ---- staging.  Wave w moves keys 16 w .. 16 w + 15 of a tile: one run of 16, so one page, whose address is scalar.  A lane
+    // adds offsets that are the same for every tile.
+    const int ch = lane % CPR, srow = lane / CPR;
     const int* const pages = p.table + (long)w.b * p.table_stride;
     const int page_mask = (1 << p.c.page_shift) - 1;
-    const int run = (wave * (64 / CPR)) >> 4;                // run of 16 keys within the first RPP rows
-    const int lane_off = (srow & 15) * (int)p.c.token_stride + ch * EPL;
-    u32x4 rk[NI], rv[NI];
-    int pg[NI], pg_s = -1;                                   // pages of the rows to be loaded next
-    unsigned ok = 0;                                         // bit i: the page of rows i of the loaded tile exists
-    float rscale = 0.f;
-    bool ok_s = false;
-    // What is loaded here and in load_tile is looked at one tile later: a comparison here would wait for every load in flight.
-    auto page_id = [&](int key) -> int { return pages[min(key, key1 - 1) >> p.c.page_shift]; };
-    auto load_pages = [&](int kv0) {
+    constexpr int ES = KV8 ? 1 : 2;                          // bytes of a value
+    unsigned lane_off[NI];
 #pragma unroll
-        for (int i = 0; i < NI; ++i) pg[i] = page_id(kv0 + 16 * run + RPP * i);
-        if constexpr (KV8) pg_s = page_id(kv0 + (tid & (KT - 1)));
-    };
+    for (int i = 0; i < NI; ++i) lane_off[i] = ((unsigned)(srow + RPL * i) * (unsigned)p.c.token_stride + ch * EPL) * ES;
+    const char* const kbase = static_cast<const char*>(p.c.k) + (long)w.g * p.c.head_stride * ES;
+    const char* const vbase = static_cast<const char*>(p.c.v) + (long)w.g * p.c.head_stride * ES;
+    u32x4 rk[NI], rv[NI];
+    int pg = -1;                                             // page of the rows to be loaded next
+    bool ok = false;                                         // the page of the loaded rows exists
+    float rscale = 0.f;
+    // What is loaded here and in load_tile is looked at one tile later: a comparison here would wait for every load in flight.
+    auto load_page = [&](int kv0) { pg = pages[min(kv0 + 16 * wave, key1 - 1) >> p.c.page_shift]; };
     auto load_tile = [&](int kv0) {
-        ok = 0;
+        const int id = __builtin_amdgcn_readfirstlane(pg);
+        ok = (unsigned)id < (unsigned)p.c.n_pages;
+        const unsigned page = ok ? id : 0, place = (kv0 + 16 * wave) & page_mask;
+        const long off = ((long)page * (unsigned)p.c.page_stride + (long)place * (unsigned)p.c.token_stride) * ES;
+        // at most 16 columns: the rows are read once, and a step moves more than the caches hold
+        auto row16 = [&](const char* at) {
+            if constexpr (QT == 1) return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at));
+            else return *reinterpret_cast<const u32x4*>(at);
+        };
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const int id = __builtin_amdgcn_readfirstlane(pg[i]);
-            const bool there = id >= 0 && id < p.c.n_pages;
-            ok |= there ? 1u << i : 0u;
-            const long base = (long)(there ? id : 0) * p.c.page_stride + w.g * p.c.head_stride + (long)((kv0 + 16 * run + RPP * i) & page_mask) * p.c.token_stride;
-            // at most 16 columns: the rows are read once, and a step moves more than the caches hold
-            auto row16 = [&](const void* at) {
-                if constexpr (QT == 1) return __builtin_nontemporal_load(static_cast<const u32x4*>(at));
-                else return *static_cast<const u32x4*>(at);
-            };
-            if constexpr (KV8) {
-                rk[i] = row16(static_cast<const uint8_t*>(p.c.k) + base + lane_off);
-                rv[i] = row16(static_cast<const uint8_t*>(p.c.v) + base + lane_off);
-            } else {
-                rk[i] = row16(static_cast<const short*>(p.c.k) + base + lane_off);
-                rv[i] = row16(static_cast<const short*>(p.c.v) + base + lane_off);
-            }
+            rk[i] = row16(kbase + off + lane_off[i]);
+            rv[i] = row16(vbase + off + lane_off[i]);
         }
-        if constexpr (KV8) {
-            ok_s = pg_s >= 0 && pg_s < p.c.n_pages && kv0 + (tid & (KT - 1)) < key1;
-            const long at = (((long)(ok_s ? pg_s : 0) * p.c.heads + w.g) << p.c.page_shift) + ((kv0 + (tid & (KT - 1))) & page_mask);
-            rscale = (tid < KT ? p.c.ks : p.c.vs)[at];       // (the upper half of the workgroup's is not used)
-        }
+        if constexpr (KV8)                                   // lanes 0..15: K's scales of the 16 rows, 16..31: V's
+            rscale = (lane & 16 ? p.c.vs : p.c.ks)[(((long)page * p.c.heads + w.g) << p.c.page_shift) + place + (lane & 15)];
     };
     auto store_tile = [&](int it) {
         const int kv0 = key0 + it * KT;
         bool bad = false;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const int row = srow + RPP * i;
+            const int row = 16 * wave + srow + RPL * i;
             if constexpr (KV8) {
                 *reinterpret_cast<short8v*>(&ldsK[k_at<D>(row, 2 * ch)]) = widen8<T>(rk[i][0], rk[i][1]);
                 *reinterpret_cast<short8v*>(&ldsK[k_at<D>(row, 2 * ch + 1)]) = widen8<T>(rk[i][2], rk[i][3]);
@@ -189,21 +178,24 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
                 lo = __builtin_bit_cast(u32x4, widen8<T>(rv[i][0], rv[i][1]));
                 hi = __builtin_bit_cast(u32x4, widen8<T>(rv[i][2], rv[i][3]));
             }
-            if (kv0 + KT > kept || !(ok >> i & 1)) {         // (uniform) tiles with rows of this step, or behind the last key
+            if (kv0 + KT > min(kept, key1) || !ok) {                    // (uniform) tiles with rows of this step, or behind the last key
                 // V's infinities and NaN are held back here: in the product they would reach rows that do not see them (0 times
                 // NaN is NaN).  The rows that do get them at the end.  What lies behind the last key may be anything.
                 const u32x4 none = {0, 0, 0, 0};
-                if (kv0 + row >= key1 || !(ok >> i & 1)) lo = hi = none;
+                if (kv0 + row >= key1 || !ok) lo = hi = none;
                 lo = finite_only<T>(lo, bad);
                 if constexpr (KV8) hi = finite_only<T>(hi, bad);
             }
             *reinterpret_cast<u32x4*>(&ldsV[v_at<D>(row, EPL * ch)]) = lo;
             if constexpr (KV8) *reinterpret_cast<u32x4*>(&ldsV[v_at<D>(row, EPL * ch + 8)]) = hi;
-            if (ch == 0 && (row & 15) == 0) lds.page_ok[row >> 4] = ok >> i & 1;
         }
+        if (lane == 0) lds.page_ok[wave] = ok;
         if (bad) lds.bad_v = 1;
         if constexpr (KV8) {
-            if (tid < 2 * KT) lds.scales[tid / KT][tid & (KT - 1)] = !ok_s ? 0.f : tid < KT ? rscale * to_log2 : rscale;
+            if (lane < 32) {
+                const bool there = ok && kv0 + 16 * wave + (lane & 15) < key1;
+                lds.scales[lane >> 4][16 * wave + (lane & 15)] = !there ? 0.f : lane < 16 ? rscale * to_log2 : rscale;
+            }
         }
     };
 
@@ -234,9 +226,9 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
     };
     if (tid == 0) lds.bad_v = 0;
     if (n_tiles > 0) {
-        load_pages(key0);
+        load_page(key0);
         load_tile(key0);
-        load_pages(key0 + KT);
+        load_page(key0 + KT);
     }
     // the queries are here before the first product: a wait for them inside the loop would be one for all loads in flight
 #pragma unroll
@@ -250,7 +242,7 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
         __syncthreads();
         if (it + 1 < n_tiles) {
             load_tile(kv0 + KT);
-            load_pages(kv0 + 2 * KT);
+            load_page(kv0 + 2 * KT);
         }
         __builtin_amdgcn_sched_barrier(0);                   // phases stay apart: mixed, their operands do not fit the registers
         if (!active) continue;

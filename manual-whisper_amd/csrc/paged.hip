@@ -54,7 +54,7 @@ int check_cache(const char* who, const mw_paged_cache* c) {
     REFUSE_IF(c->page_stride % unit || c->head_stride % unit || c->token_stride % unit || misaligned(c->k, 16) || misaligned(c->v, 16),
               "rows of the cache must start at multiples of 16 bytes");
     REFUSE_IF(c->token_stride < c->head_dim || c->head_stride < c->head_dim || c->page_stride < c->head_dim, "strides of the cache must be at least head_dim");
-    REFUSE_IF(c->token_stride > (1 << 26), "token_stride must be at most 2^26");
+    REFUSE_IF(c->token_stride > (1 << 26) || c->page_stride > UINT32_MAX, "token_stride must be at most 2^26 and page_stride below 2^32");
     return MW_OK;
 }
 int log2i(int n) { int s = 0; while ((1 << s) < n) ++s; return s; }
