@@ -74,6 +74,18 @@ __device__ __forceinline__ float column_sum(float v) {
 // pieces of 16 bytes of K, 8 of 32 bytes of V) start in different banks and every address is one register and a constant.
 template <int D> __device__ __forceinline__ int k_at(int row, int chunk) { return row * (D + 8) + chunk * 8; }
 template <int D> __device__ __forceinline__ int v_at(int row, int col) { return row * (D + 16) + col; }
+// Order of a phase of N operands from LDS (READS reads each) with M matrix instructions each: AHEAD operands first, then one
+// operand after the products of another.
+template <int N, int M, int AHEAD, int READS> __device__ __forceinline__ void interleave() {
+    constexpr int A = AHEAD < N ? AHEAD : N;
+    __builtin_amdgcn_sched_group_barrier(0x100, A * READS, 0);
+#pragma unroll
+    for (int i = 0; i < N - A; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, A * M, 0);
+}
 // 8 e4m3 codes -> 8 values of T (exact)
 template <typename T> __device__ __forceinline__ short8v widen8(unsigned a, unsigned b) {
     typedef float f2 __attribute__((ext_vector_type(2)));
@@ -260,6 +272,8 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
                 for (int qs = 0; qs < QT; ++qs) sc[i][qs] = Mat<T>::mma32(kf, qf[qs][s], sc[i][qs]);
             }
         }
+        // six operands on their way to the products throughout (left alone, the scheduler waits for every second one)
+        interleave<NK * (D / 32), QT, 6, 1>();
         __builtin_amdgcn_sched_barrier(0);
         // ---- the keys that a column does not see
         const int4 there = *reinterpret_cast<const int4*>(lds.page_ok);
@@ -387,6 +401,7 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
                         for (int qs = 0; qs < QT; ++qs) o[d][qs] = Mat<T>::mma32(vf, pf[qs][s], o[d][qs]);
                     }
             }
+            interleave<NK == 1 ? ND : ND * NK / 2, QT, 4, NK == 1 ? 1 : 2>();
         }
     }
 
