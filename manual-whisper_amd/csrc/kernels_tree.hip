@@ -537,23 +537,23 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeAttnParams p
     else attend<T, KV8, D, 2, 1>(p, group, w, lds);
 }
 
-// Rows of requests that were cut: the units' partial results, weighted by their maxima.  WAVES waves per (row, query head); their
-// groups of D / 4 lanes take the units in turn, eight loads ahead, and are joined by a butterfly, waves through LDS.
-template <typename T, int D, int WAVES>
+// Rows of requests that were cut: the units' partial results, weighted by their maxima.  D / 4 lanes hold a (row, query head),
+// four head dims each.  SHARE: a workgroup per pair whose groups of lanes take the units in turn and are joined through LDS;
+// else every group has a pair of its own.  Eight loads ahead.
+template <typename T, int D, bool SHARE>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeAttnParams p, int group) {
-    constexpr int LANES = D / 4, GROUPS = 64 / LANES, AHEAD = 8;
-    __shared__ float red_m[WAVES], red_l[WAVES];
-    __shared__ __attribute__((aligned(16))) float red_o[WAVES][D];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const long id = WAVES == 1 ? (long)blockIdx.x * 4 + wave : blockIdx.x;
+    constexpr int LANES = D / 4, GROUPS = 256 / LANES, AHEAD = 8, STEP = SHARE ? GROUPS : 1;
+    __shared__ float red_m[GROUPS], red_l[GROUPS];
+    __shared__ __attribute__((aligned(16))) float red_o[SHARE ? GROUPS : 1][D];
+    const int mine = threadIdx.x / LANES, d = (threadIdx.x % LANES) * 4;
+    const long id = SHARE ? blockIdx.x : (long)blockIdx.x * GROUPS + mine;
     const int h = (int)(id % p.heads);
     const long bi = id / p.heads;
     const int b = (int)(bi / p.max_nodes), i = (int)(bi - (long)b * p.max_nodes);
     if (b >= p.batch) return;
-    const int u0 = p.unit_start[b], n = p.unit_start[b + 1] - u0;
-    const int row = p.row_start[b] + i;
-    if (n < 2 || u0 < 0 || u0 + n > p.n_units || p.row_start[b] < 0 || row >= p.row_start[b + 1] || row >= p.rows) return;
-    const int g = h / group, part = lane / LANES + (WAVES == 1 ? 0 : wave * GROUPS), d = (lane % LANES) * 4;
+    const int u0 = p.unit_start[b], n = p.unit_start[b + 1] - u0, r0 = p.row_start[b], row = r0 + i;
+    if (n < 2 || u0 < 0 || u0 + n > p.n_units || r0 < 0 || row >= p.row_start[b + 1] || row >= p.rows) return;
+    const int g = h / group;
     const long cols = (long)p.max_nodes * group, step = p.c.heads * cols;               // slots from one unit to the next
     const long first = ((long)u0 * p.c.heads + g) * cols + (long)i * group + (h - g * group);
     const float* const po = p.workspace;
@@ -568,31 +568,28 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeAttnParams p, int gr
 #pragma unroll
         for (int r = 0; r < 4; ++r) acc[r] = acc[r] * fo + x[r] * fu;
     };
-    for (int u = part; u < n; u += GROUPS * WAVES * AHEAD) {
+    for (int u = SHARE ? mine : 0; u < n; u += STEP * AHEAD) {
         float um[AHEAD], ul[AHEAD];
         float4v x[AHEAD];
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a) {
-            const long slot = first + min(u + a * GROUPS * WAVES, n - 1) * step;
+            const long slot = first + min(u + a * STEP, n - 1) * step;
             um[a] = ml[slot * 2]; ul[a] = ml[slot * 2 + 1];
             x[a] = *reinterpret_cast<const float4v*>(po + slot * D + d);
         }
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a)
-            if (u + a * GROUPS * WAVES < n) add(um[a], ul[a], x[a]);
+            if (u + a * STEP < n) add(um[a], ul[a], x[a]);
     }
-#pragma unroll
-    for (int s = LANES; s < 64; s <<= 1)
-        add(__shfl_xor(m, s), __shfl_xor(l, s), float4v{__shfl_xor(acc[0], s), __shfl_xor(acc[1], s), __shfl_xor(acc[2], s), __shfl_xor(acc[3], s)});
-    if constexpr (WAVES > 1) {
-        if (lane == 0) { red_m[wave] = m; red_l[wave] = l; }
-        if (lane < LANES) *reinterpret_cast<float4v*>(&red_o[wave][d]) = acc;
+    if constexpr (SHARE) {
+        if (d == 0) { red_m[mine] = m; red_l[mine] = l; }
+        *reinterpret_cast<float4v*>(&red_o[mine][d]) = acc;
         __syncthreads();
+        if (mine) return;
         m = -INFINITY; l = 0.f; acc = float4v{0, 0, 0, 0};
 #pragma unroll
-        for (int k = 0; k < WAVES; ++k) add(red_m[k], red_l[k], *reinterpret_cast<const float4v*>(&red_o[k][d]));
+        for (int k = 0; k < GROUPS; ++k) add(red_m[k], red_l[k], *reinterpret_cast<const float4v*>(&red_o[k][d]));
     }
-    if (part) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     *reinterpret_cast<short4v*>(static_cast<short*>(p.out) + (long)row * p.out_row + (long)h * p.out_head + d) =
         short4v{bits_of<T>(acc[0] * inv), bits_of<T>(acc[1] * inv), bits_of<T>(acc[2] * inv), bits_of<T>(acc[3] * inv)};
@@ -609,11 +606,11 @@ void launch_tree_t(const TreeAttnParams& p, hipStream_t s) {
     if (block == 16) tree_attn_narrow_kernel<T, KV8, D><<<grid, 256, 0, s>>>(p, n_blocks, group);
     else tree_attn_wide_kernel<T, KV8, D><<<grid, 256, 0, s>>>(p, n_blocks, group);
     if (p.n_units > p.batch) {
-        // few rows have few waves: four of them share a row's units then (8 requests of 1 row, 32 heads, up to 80 units: 15.5 ->
-        // 5.5 us); for many rows one wave each is faster (32 trees, 8 units at most: 44 -> 29 us)
-        const long pairs = (long)p.batch * p.max_nodes * p.heads;
-        if (pairs <= 4096) tree_join_kernel<T, D, 4><<<(unsigned)pairs, 256, 0, s>>>(p, group);
-        else tree_join_kernel<T, D, 1><<<(unsigned)((pairs + 3) / 4), 256, 0, s>>>(p, group);
+        // few rows have few waves: a workgroup shares a row's units then (8 requests of 1 row, 32 heads, up to 80 units: 15.5 ->
+        // 5.1 us); for many rows with a pair on every group of lanes it is faster without (32 trees, 8 units at most: 44 us shared)
+        const long pairs = (long)p.batch * p.max_nodes * p.heads, groups = 256 / (D / 4);
+        if (pairs <= 4096) tree_join_kernel<T, D, true><<<(unsigned)pairs, 256, 0, s>>>(p, group);
+        else tree_join_kernel<T, D, false><<<(unsigned)((pairs + groups - 1) / groups), 256, 0, s>>>(p, group);
     }
 }
 
