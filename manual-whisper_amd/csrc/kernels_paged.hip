@@ -15,37 +15,42 @@ namespace {
 // Every workgroup computes the prefix sums over the requests for itself (at most 2048 requests, a few KB that stay in L2)
 // and then does its share of the rows, new pages, returned pages, tree masks and units: one launch without any exchange
 // between workgroups.  A page popped from a stack entry that this very step pushes is looked up in the table of the request
-// that gives it back, so pops never wait for pushes.
-constexpr int kPlanThreads = 1024;
+// that gives it back, so pops never wait for pushes.  Bound by latency: round trips to memory and the scans' barriers.
+constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 constexpr int kPlanPer = kPlanMaxBatch / kPlanThreads;       // requests per thread of the prefix sums
+constexpr unsigned kFull = 1u << 30;                         // sums of counts stop here: above every capacity, and two of them fit 32 bits
 
-__device__ __forceinline__ long wave_scan(long v) {          // inclusive, over 64 lanes
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const long o = __shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
-    return v;
+__device__ __forceinline__ unsigned sat_add(unsigned a, unsigned b) { return min(a + b, kFull); }
+template <int CTRL, int ROWS> __device__ __forceinline__ unsigned scan_step(unsigned v) {
+    return sat_add(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false));
 }
-// Exclusive prefix of `v` over the 1024 threads; `total` receives the sum.  `ws`: 17 longs of LDS.
-__device__ __forceinline__ long block_scan(long v, long* ws, long& total) {
+__device__ __forceinline__ unsigned wave_scan(unsigned v) {  // inclusive, over 64 lanes: within rows of 16, then across them
+    v = scan_step<0x111, 0xf>(v);
+    v = scan_step<0x112, 0xf>(v);
+    v = scan_step<0x114, 0xf>(v);
+    v = scan_step<0x118, 0xf>(v);
+    v = scan_step<0x142, 0xa>(v);
+    return scan_step<0x143, 0xc>(v);
+}
+// Exclusive prefixes of N counts over the workgroup's threads, and their totals.  `ws`: LDS of its own for this call.
+template <int N> __device__ __forceinline__ void block_scan(unsigned (&v)[N], unsigned (&total)[N], unsigned (*ws)[kPlanWaves]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long inc = wave_scan(v);
-    __syncthreads();                                         // ws may still be read by the previous scan
-    if (lane == 63) ws[wave] = inc;
-    __syncthreads();
-    long before = 0, sum = 0;
 #pragma unroll
-    for (int w = 0; w < kPlanThreads / 64; ++w) {
-        const long x = ws[w];
-        if (w < wave) before += x;
-        sum += x;
+    for (int k = 0; k < N; ++k) {
+        const unsigned inc = wave_scan(v[k]);
+        if (lane == 63) ws[k][wave] = inc;
+        const unsigned before = (unsigned)__shfl_up((int)inc, 1);
+        v[k] = lane ? before : 0u;
     }
-    total = sum;
-    return before + inc - v;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const unsigned w = wave_scan(lane < kPlanWaves ? ws[k][lane] : 0u);
+        total[k] = (unsigned)__shfl((int)w, kPlanWaves - 1);
+        const unsigned before = (unsigned)__shfl((int)w, max(wave - 1, 0));
+        v[k] = sat_add(v[k], wave ? before : 0u);
+    }
 }
-__device__ __forceinline__ int sat32(long v) { return v > 0x7fffffffL ? 0x7fffffff : (int)v; }
 // number of entries of the ascending array a[0..n) that are <= x
 __device__ __forceinline__ int count_le(const int* a, int n, int x) {
     int lo = 0, hi = n;
@@ -57,10 +62,12 @@ __device__ __forceinline__ int count_le(const int* a, int n, int x) {
 }
 
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) {
-    __shared__ long ws[17];
+    __shared__ unsigned ws[4][kPlanWaves];
+    __shared__ unsigned long long lens[kPlanWaves];
     __shared__ int start[kPlanMaxBatch + 1];                 // first row of each request
     __shared__ int gend[kPlanMaxBatch];                      // new pages wanted up to and including each request
     __shared__ int bend[kPlanMaxBatch];                      // pages given back up to and including each request
+    __shared__ int kept_of[kPlanMaxBatch], held_of[kPlanMaxBatch];
     __shared__ int uend[kPlanMaxBatch + 1];                  // units before each request (the last workgroup's)
     __shared__ unsigned char state[kPlanMaxBatch];           // 1 = valid, 2 = admitted
     __shared__ unsigned anc[32 * kPlanMaxWords][kPlanMaxWords + 1];
@@ -69,125 +76,102 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
     const int page = 1 << p.page_shift;
 
     // ---- prefix sums over the requests
-    long kept[kPlanPer], fresh[kPlanPer];
-    int held[kPlanPer];
-    long sum = 0;
+    int kept[kPlanPer], fresh[kPlanPer], held[kPlanPer];
+    unsigned rows[1] = {0}, total_rows[1];
+    const int n_free = min(max(p.n_free_in[0], 0), p.n_pages);
 #pragma unroll
     for (int i = 0; i < kPlanPer; ++i) {
         const int b = tid * kPlanPer + i;
         kept[i] = b < B ? p.kept[b] : 0;
         fresh[i] = b < B ? p.fresh[b] : 0;
         held[i] = b < B ? min(max(p.pages_in[b], 0), p.max_pages) : 0;
-        sum += fresh[i] > 0 ? fresh[i] : 0;
+        rows[0] = sat_add(rows[0], min((unsigned)max(fresh[i], 0), kFull));
     }
-    long total_rows;
-    long at = block_scan(sum, ws, total_rows);
-    long grow[kPlanPer], back[kPlanPer], need[kPlanPer];
+    block_scan<1>(rows, total_rows, ws);
+    int need[kPlanPer];
+    unsigned grow[kPlanPer], back[kPlanPer], both[2] = {0, 0}, total[2];
     bool valid[kPlanPer];
-    long gsum = 0, bsum = 0;
 #pragma unroll
     for (int i = 0; i < kPlanPer; ++i) {
         const int b = tid * kPlanPer + i;
-        if (b < B) start[b] = sat32(at);
-        at += fresh[i] > 0 ? fresh[i] : 0;
-        need[i] = (kept[i] + fresh[i] + page - 1) >> p.page_shift;
-        valid[i] = b < B && kept[i] >= 0 && fresh[i] >= 0 && need[i] <= p.max_pages && at <= p.rows &&
+        if (b < B) { start[b] = (int)rows[0]; kept_of[b] = kept[i]; held_of[b] = held[i]; }
+        rows[0] = sat_add(rows[0], min((unsigned)max(fresh[i], 0), kFull));
+        const long pages = ((long)kept[i] + fresh[i] + page - 1) >> p.page_shift;
+        valid[i] = b < B && kept[i] >= 0 && fresh[i] >= 0 && pages <= p.max_pages && rows[0] <= (unsigned)p.rows &&
                    (!p.parents || fresh[i] <= 32 * p.mask_words);
+        need[i] = valid[i] ? (int)pages : 0;
         grow[i] = valid[i] && need[i] > held[i] ? need[i] - held[i] : 0;
         back[i] = valid[i] && need[i] < held[i] ? held[i] - need[i] : 0;
-        gsum += grow[i]; bsum += back[i];
+        both[0] = sat_add(both[0], grow[i]); both[1] = sat_add(both[1], back[i]);
     }
-    if (tid == 0) start[B] = sat32(total_rows);
-    long total_grow, total_back;
-    long gat = block_scan(gsum, ws, total_grow);
-    long bat = block_scan(bsum, ws, total_back);
-    const int n_free = min(max(p.n_free_in[0], 0), p.n_pages);
-    const long stack = n_free + total_back;                  // pages to be had in this step
-    long used = 0, len_sum = 0;
-    long len[kPlanPer];
+    if (tid == 0) start[B] = (int)total_rows[0];
+    block_scan<2>(both, total, ws + 1);
+    const unsigned stack = n_free + total[1];                // pages to be had in this step
+    unsigned used = 0;                                       // growing requests are admitted up to some point and none behind it
+    unsigned long long len_sum = 0;
+    int len[kPlanPer];
 #pragma unroll
     for (int i = 0; i < kPlanPer; ++i) {
         const int b = tid * kPlanPer + i;
-        gat += grow[i]; bat += back[i];
-        const bool admitted = valid[i] && (grow[i] == 0 || gat <= stack);
+        both[0] = sat_add(both[0], grow[i]); both[1] = sat_add(both[1], back[i]);
+        const bool admitted = valid[i] && (grow[i] == 0 || both[0] <= stack);
         if (b < B) {
-            gend[b] = sat32(gat); bend[b] = sat32(bat);
+            gend[b] = (int)both[0]; bend[b] = (int)both[1];
             state[b] = (valid[i] ? 1 : 0) | (admitted ? 2 : 0);
             if (blockIdx.x == 0) {
                 p.row_start[b] = start[b];
                 p.admitted[b] = admitted;
-                p.pages_out[b] = admitted ? (int)need[i] : held[i];
+                p.pages_out[b] = admitted ? need[i] : held[i];
             }
         }
-        if (admitted) used += grow[i];
+        if (admitted && grow[i]) used = both[0];
         len[i] = admitted && fresh[i] > 0 ? kept[i] + fresh[i] : 0;
-        len_sum += len[i];
+        len_sum += (unsigned)len[i];
     }
-    long total_used, total_len;
-    block_scan(used, ws, total_used);
-    block_scan(len_sum, ws, total_len);
-    if (blockIdx.x == 0 && tid == 0) {
-        p.row_start[B] = start[B];
-        p.n_free_out[0] = (int)min(stack - total_used, (long)p.n_pages);
+    // largest `used`, sum of the lengths
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        used = max(used, (unsigned)__shfl_xor((int)used, d));
+        len_sum += __shfl_xor(len_sum, d);
     }
+    if ((tid & 63) == 0) { ws[3][tid >> 6] = used; lens[tid >> 6] = len_sum; }
     __syncthreads();
+    if (blockIdx.x == 0 && tid == 0) {
+        for (int w = 1; w < kPlanWaves; ++w) used = max(used, ws[3][w]);
+        p.row_start[B] = start[B];
+        p.n_free_out[0] = (int)min(stack - used, (unsigned)p.n_pages);
+    }
 
     // page on top of entry `e` of the stack as this step's pushes leave it
-    auto stack_page = [&](long e) -> int {
+    auto stack_page = [&](int e) -> int {
         if (e < n_free) return p.free_list[e];
-        const int k = sat32(e - n_free), b = min(count_le(bend, B, k), B - 1);
-        const int first = (int)((p.kept[b] + (long)p.fresh[b] + page - 1) >> p.page_shift);
+        const int k = e - n_free, b = min(count_le(bend, B, k), B - 1);
+        const int first = held_of[b] - (bend[b] - (b ? bend[b - 1] : 0));                // what request b keeps
         return p.table[(long)b * p.table_stride + first + (k - (b ? bend[b - 1] : 0))];
     };
     // page `n` of admitted request b, old or new
     auto page_of = [&](int b, int n) -> int {
-        const int h = min(max(p.pages_in[b], 0), p.max_pages);
+        const int h = held_of[b];
         if (n < h) return p.table[(long)b * p.table_stride + n];
-        return stack_page(stack - 1 - ((b ? gend[b - 1] : 0) + (n - h)));
+        return stack_page((int)stack - 1 - ((b ? gend[b - 1] : 0) + (n - h)));
+    };
+    auto slot_of = [&](int b, int place) -> long {
+        const int pg = page_of(b, place >> p.page_shift);
+        return pg >= 0 ? ((long)pg << p.page_shift) + (place & (page - 1)) : -1;
     };
     const long threads = (long)gridDim.x * kPlanThreads, me = (long)blockIdx.x * kPlanThreads + tid;
 
-    // ---- rows: slots, and positions of chains
-    for (long r = me; r < p.rows; r += threads) {
-        long slot = -1;
-        int pos = -1;
-        bool masked = p.parents != nullptr;                  // no tree is going to write this row's mask
-        if (r < start[B]) {
-            const int b = count_le(start, B + 1, (int)r) - 1;
-            const int i = (int)r - start[b];
-            const int kb = p.kept[b];
-            if (state[b] & 1) { pos = kb + i; masked = false; }
-            if (state[b] & 2) {
-                const int place = kb + i;
-                const int pg = page_of(b, place >> p.page_shift);
-                slot = pg >= 0 ? ((long)pg << p.page_shift) + (place & (page - 1)) : -1;
-            }
-        }
-        p.slots[r] = slot;
-        if (!p.parents || masked) p.positions[r] = pos;
-        if (masked)
-            for (int w = 0; w < p.mask_words; ++w) p.mask[r * p.mask_words + w] = 0;
-    }
-    // ---- new pages into the tables, returned pages onto the stack
-    const long grown = total_grow < stack ? total_grow : stack;
-    for (long k = me; k < grown; k += threads) {
-        const int b = min(count_le(gend, B, (int)k), B - 1);
-        if (!(state[b] & 2)) continue;
-        const int h = min(max(p.pages_in[b], 0), p.max_pages);
-        p.table[(long)b * p.table_stride + h + ((int)k - (b ? gend[b - 1] : 0))] = stack_page(stack - 1 - k);
-    }
-    for (long k = me; k < total_back; k += threads)
-        if (n_free + k < p.n_pages) p.free_list[n_free + k] = stack_page(n_free + k);
-
-    // ---- trees: ancestors by pointer doubling.  Node i starts with {i} and its parent; a round adds the ancestors that its
-    // jump target has gathered and jumps on from there: log2(depth) rounds, all nodes at once.
+    // ---- trees: a workgroup per request.  Ancestors by pointer doubling: node i starts with {i} and its parent; a round adds
+    // the ancestors that its jump target has gathered and jumps on from there: log2(depth) rounds, all nodes at once.
     if (p.parents && (int)blockIdx.x < B && (state[blockIdx.x] & 1)) {
         const int b = blockIdx.x, n = start[b + 1] - start[b], W = p.mask_words;
+        const long r = start[b] + tid;
         if (tid < n) {
-            int up = p.parents[start[b] + tid];
+            int up = p.parents[r];
             if (up < 0 || up >= tid) up = -1;                // a parent is an earlier node of the same tree
             jump[tid] = up;
             for (int w = 0; w < W; ++w) anc[tid][w] = (tid >> 5) == w ? 1u << (tid & 31) : 0u;
+            p.slots[r] = (state[b] & 2) ? slot_of(b, kept_of[b] + tid) : -1;
         }
         bool more = true;
         while (more) {
@@ -211,43 +195,66 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
         }
         if (tid < n) {
             int depth = -1;
-            const long r = start[b] + tid;
             for (int w = 0; w < W; ++w) { p.mask[r * W + w] = anc[tid][w]; depth += __popc(anc[tid][w]); }
-            p.positions[r] = p.kept[b] + depth;
+            p.positions[r] = kept_of[b] + depth;
         }
     }
 
+    // ---- rows of chains; in a step of trees the rows that belong to none of them
+    for (long r = me; r < p.rows; r += threads) {
+        long slot = -1;
+        int pos = -1;
+        if (r < start[B]) {
+            const int b = count_le(start, B + 1, (int)r) - 1;
+            if (state[b] & 1) {
+                if (p.parents) continue;
+                pos = kept_of[b] + (int)r - start[b];
+            }
+            if (state[b] & 2) slot = slot_of(b, pos);
+        }
+        p.slots[r] = slot;
+        p.positions[r] = pos;
+        if (p.parents)
+            for (int w = 0; w < p.mask_words; ++w) p.mask[r * p.mask_words + w] = 0;
+    }
+    // ---- new pages into the tables, returned pages onto the stack
+    const long grown = min(total[0], stack);
+    for (long k = me; k < grown; k += threads) {
+        const int b = min(count_le(gend, B, (int)k), B - 1);
+        if (!(state[b] & 2)) continue;
+        p.table[(long)b * p.table_stride + held_of[b] + ((int)k - (b ? gend[b - 1] : 0))] = stack_page((int)stack - 1 - (int)k);
+    }
+    for (long k = me; k < total[1]; k += threads)
+        if (n_free + k < p.n_pages) p.free_list[n_free + k] = stack_page(n_free + (int)k);
+
     // ---- work units of the attention
     if (p.units && blockIdx.x == gridDim.x - 1) {
-        long most = p.chunk_units ? (total_len + p.chunk_units - 1) / p.chunk_units : total_len;
-        most = (most + 63) / 64 * 64;
-        const long least = ((long)p.chunk_min + 63) / 64 * 64;
-        most = most > least ? most : least;
-        long cnt[kPlanPer], csum = 0;
+        unsigned long long total_len = 0;
+        for (int w = 0; w < kPlanWaves; ++w) total_len += lens[w];
+        unsigned long long most = p.chunk_units ? (total_len + p.chunk_units - 1) / p.chunk_units : total_len;
+        most = max((most + 63) / 64 * 64, ((unsigned long long)p.chunk_min + 63) / 64 * 64);
+        unsigned cnt[kPlanPer], sum[1] = {0}, total_units[1];
 #pragma unroll
         for (int i = 0; i < kPlanPer; ++i) {
-            const long c = (len[i] + most - 1) / most;
-            cnt[i] = fresh[i] > 0 ? (c > 1 ? c : 1) : 0;
-            csum += cnt[i];
+            cnt[i] = fresh[i] > 0 ? max((unsigned)(((unsigned long long)(unsigned)len[i] + most - 1) / most), 1u) : 0u;
+            sum[0] += cnt[i];
         }
-        long total_units;
-        long uat = block_scan(csum, ws, total_units);
+        block_scan<1>(sum, total_units, ws);
 #pragma unroll
         for (int i = 0; i < kPlanPer; ++i) {
             const int b = tid * kPlanPer + i;
-            if (b < B) { uend[b] = sat32(uat); p.unit_start[b] = sat32(uat); }
-            uat += cnt[i];
+            if (b < B) { uend[b] = (int)sum[0]; p.unit_start[b] = (int)sum[0]; }
+            sum[0] += cnt[i];
         }
-        if (tid == 0) { uend[B] = sat32(total_units); p.unit_start[B] = sat32(total_units); }
+        if (tid == 0) { uend[B] = (int)total_units[0]; p.unit_start[B] = (int)total_units[0]; }
         __syncthreads();
         for (int u = tid; u < B + p.chunk_units; u += kPlanThreads) {
             int4 unit = make_int4(-1, -1, -1, -1);
             if (u < uend[B]) {
                 const int b = count_le(uend, B + 1, u) - 1, n = uend[b + 1] - uend[b];
-                const long l = (state[b] & 2) ? p.kept[b] + (long)p.fresh[b] : 0;
-                const long each = ((l + n - 1) / n + 63) / 64 * 64;
-                const long first = (u - uend[b]) * each;
-                unit = make_int4(b, (int)min(first, l), (int)min(first + each, l), n);
+                const int l = (state[b] & 2) ? kept_of[b] + (start[b + 1] - start[b]) : 0;
+                const long each = (((long)l + n - 1) / n + 63) / 64 * 64, first = (u - uend[b]) * each;
+                unit = make_int4(b, (int)min(first, (long)l), (int)min(first + each, (long)l), n);
             }
             reinterpret_cast<int4*>(p.units)[u] = unit;
         }
@@ -281,9 +288,18 @@ template <bool BF, int LPR> __device__ __forceinline__ uint2 quant8(uint4 u, flo
     for (int d = 1; d < LPR; d <<= 1) big = max(big, (unsigned)__shfl_xor((int)big, d));
     // a row with an infinity or a NaN has no scale: it comes back as NaN throughout
     scale = big >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float(big) / 448.f;
-    const float by = scale > 0.f ? scale : 1.f;
+    if (scale > 0x1p-100f) {                                 // quotients to the last bit: a product and one correction
+        const float inv = 1.f / scale;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = f[i] / by;
+        for (int i = 0; i < 8; ++i) {
+            const float q = f[i] * inv;
+            f[i] = fmaf(fmaf(-q, scale, f[i]), inv, q);
+        }
+    } else {
+        const float by = scale > 0.f ? scale : 1.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = f[i] / by;
+    }
     return make_uint2(pack4_e4m3(f[0], f[1], f[2], f[3]), pack4_e4m3(f[4], f[5], f[6], f[7]));
 }
 
@@ -348,16 +364,29 @@ __global__ __launch_bounds__(256) void accept_scan_kernel(const T* __restrict__ 
     const int lead = (int)(((16 - (reinterpret_cast<uintptr_t>(x + v0) & 15)) & 15) / sizeof(T));
     const int a0 = min(v1, v0 + lead), nvec = (v1 - a0) / VEC;
     if (v0 + (int)threadIdx.x < a0) take(logit_f32<T>(x[v0 + threadIdx.x]), v0 + threadIdx.x);
-    const uint4* body = reinterpret_cast<const uint4*>(x + a0);
-    for (int j = threadIdx.x; j < nvec; j += 256) {
-        const uint4 u = body[j];
-        const T* e = reinterpret_cast<const T*>(&u);
-        float m = logit_f32<T>(e[0]);
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    const u32x4* body = reinterpret_cast<const u32x4*>(x + a0);
+    constexpr int AHEAD = 8;
+    for (int j0 = threadIdx.x; j0 < nvec; j0 += 256 * AHEAD) {
+        u32x4 u[AHEAD];                                      // read once: nothing is gained by keeping them in the caches
 #pragma unroll
-        for (int i = 1; i < VEC; ++i) m = fmaxf(m, logit_f32<T>(e[i]));
-        if (m > best.v) {
+        for (int a = 0; a < AHEAD; ++a) u[a] = __builtin_nontemporal_load(body + min(j0 + 256 * a, nvec - 1));
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) take(logit_f32<T>(e[i]), a0 + j * VEC + i);
+        for (int a = 0; a < AHEAD; ++a) {
+            const int j = j0 + 256 * a;
+            float f[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                if constexpr (sizeof(T) == 4) f[i] = __uint_as_float(u[a][i]);
+                else f[i] = logit_f32<T>(__builtin_bit_cast(T, (unsigned short)(u[a][i >> 1] >> (16 * (i & 1)))));
+            }
+            float m = f[0];
+#pragma unroll
+            for (int i = 1; i < VEC; ++i) m = fmaxf(m, f[i]);
+            if (j < nvec && m > best.v) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) take(f[i], a0 + j * VEC + i);
+            }
         }
     }
     const int tail = a0 + nvec * VEC + threadIdx.x;
@@ -384,7 +413,14 @@ __global__ __launch_bounds__(256) void accept_walk_kernel(AcceptParams p, int pa
     const int n = max(0, min(r1 - r0, p.depth));
     for (int i = threadIdx.x; i < max(0, r1 - r0); i += 256) {
         Best best{-INFINITY, 0x7fffffff};
-        for (int k = 0; k < parts; ++k) best = better(best, Best{part_v[(long)(r0 + i) * parts + k], part_i[(long)(r0 + i) * parts + k]});
+        const long at = (long)(r0 + i) * parts;
+        for (int k0 = 0; k0 < parts; k0 += 8) {
+            Best x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = Best{part_v[at + min(k0 + k, parts - 1)], part_i[at + min(k0 + k, parts - 1)]};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) best = better(best, x[k]);
+        }
         const int id = best.i == 0x7fffffff ? 0 : best.i;    // nothing to choose from: the lowest id
         p.best[r0 + i] = id;
         if (i < n) { ids[i] = id; next[i] = 0x7fffffff; }
@@ -408,78 +444,88 @@ __global__ __launch_bounds__(256) void accept_walk_kernel(AcceptParams p, int pa
 }
 
 // -------------------------------------------------------------------------------------------- compact
-// A thread owns 16 bytes of a (layer, head, K or V) column and moves them for every accepted node: HBM-bound, 16 bytes in
-// and out per piece.  A path ascends and path[i] >= i, so a row that is written is never one that is still to be read:
-// the reads of eight nodes are issued together.
+// A workgroup owns up to 128 pieces of 16 bytes of a layer's token rows (heads of K, heads of V, and the row scales as pieces
+// of 4) and moves them for every accepted node: HBM-bound, 16 bytes in and out per piece.  A path ascends and path[i] >= i, so
+// what move i overwrites is only ever read by moves before it: a batch of moves is read as a whole, then written.
+constexpr int kCompactPieces = 128, kCompactPer = 8;
+template <typename V> __device__ __forceinline__ void move_pieces(char* const* column, int pieces, const long* src, const long* dst, int moves) {
+    // item e = (move, piece), neighbours in a row side by side; kCompactPer items per thread are in flight
+    const unsigned inv = (1u << 20) / pieces + 1;            // e / pieces = e * inv >> 20, exact for e < 2048 and pieces <= 128
+    const int per = 256 * kCompactPer / pieces;
+    for (int j0 = 0; j0 < moves; j0 += per) {
+        const int items = min(moves - j0, per) * pieces;
+        V v[kCompactPer];
+        char* to[kCompactPer];
+#pragma unroll
+        for (int a = 0; a < kCompactPer; ++a) {
+            const int e = threadIdx.x + 256 * a, j = (int)(e * inv >> 20);
+            if (e >= items) continue;
+            char* const at = column[e - j * pieces];
+            v[a] = *reinterpret_cast<const V*>(at + src[j0 + j]);
+            to[a] = at + dst[j0 + j];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int a = 0; a < kCompactPer; ++a)
+            if ((int)threadIdx.x + 256 * a < items) *reinterpret_cast<V*>(to[a]) = v[a];
+    }
+}
 __global__ __launch_bounds__(256) void paged_compact_kernel(PagedCacheView c, long layer_stride, long scale_layer_stride, int esize, int dim,
                                                             const int* __restrict__ table, long table_stride, int max_pages,
                                                             const int* __restrict__ kept, const int* __restrict__ path, int path_cols,
                                                             const int* __restrict__ count) {
-    constexpr int PER = 8;
-    __shared__ int src[256], dst[256];                       // slots of up to 256 moves; -1: nothing to move
-    __shared__ int n_moves;
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    __shared__ char* column[kCompactPieces];                 // where piece e of token 0 of page 0 lies
+    __shared__ long src[2][256], dst[2][256];                // byte offsets of up to 256 moves; [1]: of the scales
+    __shared__ int wsum[4];
     const int b = blockIdx.z, layer = blockIdx.y;
-    const int m = min(max(count[b], 0), path_cols);
+    const int m = min(max(count[b], 0), path_cols), kept_b = kept[b];
     const int per_row = dim * esize / 16;                    // pieces of a (head, token) row
-    const int pieces = 2 * c.heads * per_row, scales = c.ks ? 2 * c.heads : 0;
-    const int id = blockIdx.x * 256 + threadIdx.x;
+    const int all = 2 * c.heads * per_row, scale_blocks = c.ks ? (2 * c.heads + kCompactPieces - 1) / kCompactPieces : 0;
+    const bool scales = (int)blockIdx.x >= (int)gridDim.x - scale_blocks;
+    const int first = (scales ? blockIdx.x - (gridDim.x - scale_blocks) : blockIdx.x) * kCompactPieces;
+    const int pieces = min((scales ? 2 * c.heads : all) - first, kCompactPieces);
     const int page = 1 << c.page_shift;
-    auto slot_of = [&](long place) -> int {
+    for (int e = threadIdx.x; e < pieces; e += 256) {
+        const int q = first + e;
+        if (scales) {
+            const int which = q / c.heads, h = q - which * c.heads;
+            column[e] = reinterpret_cast<char*>((which ? c.vs : c.ks) + layer * scale_layer_stride + (long)h * page);
+        } else {
+            const int which = q / (c.heads * per_row), rest = q - which * c.heads * per_row, h = rest / per_row;
+            column[e] = static_cast<char*>(which ? c.v : c.k) + (layer * layer_stride + h * c.head_stride) * esize + (rest - h * per_row) * 16;
+        }
+    }
+    auto page_of = [&](long place) -> int {
         const long n = place >> c.page_shift;
         if (place < 0 || n >= max_pages) return -1;
         const int pg = table[b * table_stride + n];
-        return pg >= 0 && pg < c.n_pages ? (int)((pg << c.page_shift) + (place & (page - 1))) : -1;
+        return pg >= 0 && pg < c.n_pages ? pg : -1;
     };
     for (int i0 = 0; i0 < m; i0 += 256) {
-        __syncthreads();
-        if (threadIdx.x == 0) n_moves = 0;
-        __syncthreads();
-        const int i = i0 + threadIdx.x;
-        int s = -1, d = -1;
-        if (i < m) {
-            const int node = path[(long)b * path_cols + i];
-            if (node > i) { s = slot_of((long)kept[b] + node); d = slot_of((long)kept[b] + i); }
-        }
-        const bool move = s >= 0 && d >= 0;
+        const int i = i0 + threadIdx.x, node = i < m ? path[(long)b * path_cols + i] : -1;
+        const long from = (long)kept_b + node, to = (long)kept_b + i;
+        const int ps = node > i ? page_of(from) : -1, pd = node > i ? page_of(to) : -1;
+        const bool move = ps >= 0 && pd >= 0;
         // the moves in path order, without the nodes that lie in their place already
         const unsigned long long ball = __ballot(move);
-        const int before = __popcll(ball & ((1ull << (threadIdx.x & 63)) - 1));
-        __shared__ int wsum[4];
-        if ((threadIdx.x & 63) == 0) wsum[threadIdx.x >> 6] = __popcll(ball);
+        const int before = __popcll(ball & ((1ull << (threadIdx.x & 63)) - 1)), wave = threadIdx.x >> 6;
+        __syncthreads();                                     // the previous batch is done with src and dst
+        if ((threadIdx.x & 63) == 0) wsum[wave] = __popcll(ball);
         __syncthreads();
         int base = 0;
-        for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) base += wsum[w];
-        if (move) { src[base + before] = s; dst[base + before] = d; }
-        if (threadIdx.x == 0) n_moves = wsum[0] + wsum[1] + wsum[2] + wsum[3];
-        __syncthreads();
-        const int moves = n_moves;
-        if (id < pieces) {
-            const int which = id / (c.heads * per_row), rest = id - which * c.heads * per_row;
-            const int h = rest / per_row, piece = rest - h * per_row;
-            char* base_p = static_cast<char*>(which ? c.v : c.k) + (layer * layer_stride + h * c.head_stride) * esize + piece * 16;
-            for (int j0 = 0; j0 < moves; j0 += PER) {
-                uint4 u[PER];
-                char* to[PER];
-#pragma unroll
-                for (int j = 0; j < PER; ++j) {
-                    const int jj = min(j0 + j, moves - 1), sl = src[jj], dl = dst[jj];
-                    const char* from = base_p + ((long)(sl >> c.page_shift) * c.page_stride + (sl & (page - 1)) * c.token_stride) * esize;
-                    to[j] = base_p + ((long)(dl >> c.page_shift) * c.page_stride + (dl & (page - 1)) * c.token_stride) * esize;
-                    u[j] = *reinterpret_cast<const uint4*>(from);
-                }
-#pragma unroll
-                for (int j = 0; j < PER; ++j)
-                    if (j0 + j < moves) *reinterpret_cast<uint4*>(to[j]) = u[j];
-            }
-        } else if (id < pieces + scales) {
-            const int which = (id - pieces) / c.heads, h = (id - pieces) - which * c.heads;
-            float* s32 = (which ? c.vs : c.ks) + layer * scale_layer_stride;
-            for (int j = 0; j < moves; ++j) {
-                const int sl = src[j], dl = dst[j];
-                s32[(((long)(dl >> c.page_shift) * c.heads + h) << c.page_shift) + (dl & (page - 1))] =
-                    s32[(((long)(sl >> c.page_shift) * c.heads + h) << c.page_shift) + (sl & (page - 1))];
-            }
+        for (int w = 0; w < wave; ++w) base += wsum[w];
+        if (move) {
+            const int os = (int)(from & (page - 1)), od = (int)(to & (page - 1));
+            src[0][base + before] = (ps * c.page_stride + os * c.token_stride) * esize;
+            dst[0][base + before] = (pd * c.page_stride + od * c.token_stride) * esize;
+            src[1][base + before] = (((long)ps * c.heads << c.page_shift) + os) * 4;
+            dst[1][base + before] = (((long)pd * c.heads << c.page_shift) + od) * 4;
         }
+        const int moves = wsum[0] + wsum[1] + wsum[2] + wsum[3];
+        __syncthreads();
+        if (scales) move_pieces<unsigned>(column, pieces, src[1], dst[1], moves);
+        else move_pieces<u32x4>(column, pieces, src[0], dst[0], moves);
     }
 }
 
@@ -530,9 +576,10 @@ void launch_paged_compact(const PagedCacheView& c, int layers, long layer_stride
                           long table_stride, int max_pages, const int* kept, const int* path, int path_cols, const int* count, int batch,
                           hipStream_t s) {
     const int esize = c.ks ? 1 : 2;
-    const int threads = 2 * c.heads * (dim * esize / 16) + (c.ks ? 2 * c.heads : 0);
-    paged_compact_kernel<<<dim3((threads + 255) / 256, layers, batch), 256, 0, s>>>(c, layer_stride, scale_layer_stride, esize, dim, table,
-                                                                                    table_stride, max_pages, kept, path, path_cols, count);
+    const int blocks = (2 * c.heads * (dim * esize / 16) + kCompactPieces - 1) / kCompactPieces +
+                       (c.ks ? (2 * c.heads + kCompactPieces - 1) / kCompactPieces : 0);
+    paged_compact_kernel<<<dim3(blocks, layers, batch), 256, 0, s>>>(c, layer_stride, scale_layer_stride, esize, dim, table, table_stride, max_pages,
+                                                                     kept, path, path_cols, count);
 }
 
 }  // namespace mw

@@ -68,7 +68,7 @@ extern "C" int mw_paged_plan(const mw_plan_args* a, int device, void* stream) {
     const char* who = "mw_paged_plan";
     REFUSE_IF(!a, "null argument");
     REFUSE_IF(a->batch < 1 || a->batch > kPlanMaxBatch, "batch must be in 1.." + std::to_string(kPlanMaxBatch));
-    REFUSE_IF(a->rows < 0 || a->rows > (1 << 30), "rows must be in 0..2^30");
+    REFUSE_IF(a->rows < 0 || a->rows >= (1 << 30), "rows must be in 0..2^30 - 1");
     REFUSE_IF(a->page_size < 16 || a->page_size > 4096 || (a->page_size & (a->page_size - 1)), "page_size must be a power of two in 16..4096");
     REFUSE_IF(a->max_pages < 1 || (int64_t)a->max_pages * a->page_size > INT32_MAX, "max_pages must be at least 1 and a request hold less than 2^31 tokens");
     REFUSE_IF(a->table_stride < a->max_pages, "table_stride must be at least max_pages");

@@ -133,33 +133,30 @@ class StepPlan:
     """What ``PagePool.plan`` made: row_start [batch + 1], slots (int64) and positions [rows], mask [rows, words] (None: chains),
     admitted, pages [batch], n_free [1], units [batch + chunks, 4], unit_start [batch + 1]; int32, views of one buffer."""
 
+    _NAMES = ("units", "slots", "row_start", "admitted", "pages", "n_free", "unit_start", "positions", "mask")
+
     def __init__(self, batch: int, rows: int, words: int, n_units: int, device):
         self.batch, self.rows, self.words, self.n_units = batch, rows, words, n_units
-        at = 0
-        self._at = {}
-        for name, n in (("units", 4 * n_units), ("slots", 2 * rows), ("row_start", batch + 1), ("admitted", batch), ("pages", batch),
-                        ("n_free", 1), ("unit_start", batch + 1), ("positions", rows), ("mask", rows * words)):
-            self._at[name] = (at, n)
-            at += n
-        self._buf = torch.empty(at, dtype=_INT, device=device)
-        self._base = self._buf.data_ptr()
+        self._sizes = (4 * n_units, 2 * rows, batch + 1, batch, batch, 1, batch + 1, rows, rows * words)
+        self._buf = torch.empty(sum(self._sizes), dtype=_INT, device=device)
+        self._parts = None
 
-    def _addr(self, name: str) -> int:
-        return self._base + 4 * self._at[name][0]
+    def _addresses(self):
+        at, out = self._buf.data_ptr(), []
+        for n in self._sizes:
+            out.append(at)
+            at += 4 * n
+        return out
 
-    def _part(self, name: str):
-        at, n = self._at[name]
-        return self._buf[at:at + n]
-
-    row_start = property(lambda s: s._part("row_start"))
-    admitted = property(lambda s: s._part("admitted"))
-    pages = property(lambda s: s._part("pages"))
-    n_free = property(lambda s: s._part("n_free"))
-    unit_start = property(lambda s: s._part("unit_start"))
-    positions = property(lambda s: s._part("positions"))
-    slots = property(lambda s: s._part("slots").view(torch.int64))
-    units = property(lambda s: s._part("units").view(s.n_units, 4))
-    mask = property(lambda s: s._part("mask").view(s.rows, s.words) if s.words else None)
+    def __getattr__(self, name: str):            # the views are made when the first one is asked for
+        if name not in self._NAMES:
+            raise AttributeError(name)
+        if self._parts is None:
+            p = dict(zip(self._NAMES, self._buf.split(self._sizes)))
+            p["units"], p["slots"] = p["units"].view(self.n_units, 4), p["slots"].view(torch.int64)
+            p["mask"] = p["mask"].view(self.rows, self.words) if self.words else None
+            self._parts = p
+        return self._parts[name]
 
 
 class PagePool:
@@ -194,11 +191,10 @@ class PagePool:
         k, f = _array(kept, "kept", _INT, (self.batch,), dev), _array(fresh, "fresh", _INT, (self.batch,), dev)
         up = None if parents is None else _array(parents, "parents", _INT, (rows,), dev)
         p = StepPlan(self.batch, rows, words, self.batch + units, self.table.device)
-        at = p._addr
+        at_units, at_slots, at_start, at_admitted, at_pages, at_free, at_first, at_positions, at_mask = p._addresses()
         args = _lib.PlanArgs(self.batch, rows, self.page_size, self.free.shape[0], self.max_pages, k, f, up, self.table.data_ptr(),
-                             self.table.stride(0), self.pages.data_ptr(), at("pages"), self.free.data_ptr(), self.n_free.data_ptr(), at("n_free"),
-                             at("row_start"), at("admitted"), at("slots"), at("positions"), at("mask") if words else None, words, at("units"),
-                             at("unit_start"), units, chunk)
+                             self.table.stride(0), self.pages.data_ptr(), at_pages, self.free.data_ptr(), self.n_free.data_ptr(), at_free, at_start,
+                             at_admitted, at_slots, at_positions, at_mask if words else None, words, at_units, at_first, units, chunk)
         _check(_lib.load().mw_paged_plan(C.byref(args), dev, _stream(dev)), "mw_paged_plan")
         return p
 
