@@ -7,6 +7,8 @@
 // against its buffer before it is used.
 #include "mw_kernels.h"
 
+#include <algorithm>
+
 namespace mw {
 
 namespace {
@@ -444,13 +446,13 @@ __global__ __launch_bounds__(256) void accept_walk_kernel(AcceptParams p, int pa
 }
 
 // -------------------------------------------------------------------------------------------- compact
-// A workgroup owns up to 128 pieces of 16 bytes of a layer's token rows (heads of K, heads of V, and the row scales as pieces
+// A workgroup owns up to 64 pieces of 16 bytes of a layer's token rows (heads of K, heads of V, and the row scales as pieces
 // of 4) and moves them for every accepted node: HBM-bound, 16 bytes in and out per piece.  A path ascends and path[i] >= i, so
 // what move i overwrites is only ever read by moves before it: a batch of moves is read as a whole, then written.
-constexpr int kCompactPieces = 128, kCompactPer = 8;
-template <typename V> __device__ __forceinline__ void move_pieces(char* const* column, int pieces, const long* src, const long* dst, int moves) {
+constexpr int kCompactPieces = 64, kCompactPer = 4;
+template <typename V> __device__ __forceinline__ void move_pieces(char* const* column, int pieces, const long* src, const long* dst, int moves, long layer_off) {
     // item e = (move, piece), neighbours in a row side by side; kCompactPer items per thread are in flight
-    const unsigned inv = (1u << 20) / pieces + 1;            // e / pieces = e * inv >> 20, exact for e < 2048 and pieces <= 128
+    const unsigned inv = (1u << 20) / pieces + 1;            // e / pieces = e * inv >> 20, exact for e < 1024 and pieces <= 64
     const int per = 256 * kCompactPer / pieces;
     for (int j0 = 0; j0 < moves; j0 += per) {
         const int items = min(moves - j0, per) * pieces;
@@ -460,7 +462,7 @@ template <typename V> __device__ __forceinline__ void move_pieces(char* const* c
         for (int a = 0; a < kCompactPer; ++a) {
             const int e = threadIdx.x + 256 * a, j = (int)(e * inv >> 20);
             if (e >= items) continue;
-            char* const at = column[e - j * pieces];
+            char* const at = column[e - j * pieces] + layer_off;
             v[a] = *reinterpret_cast<const V*>(at + src[j0 + j]);
             to[a] = at + dst[j0 + j];
         }
@@ -473,12 +475,12 @@ template <typename V> __device__ __forceinline__ void move_pieces(char* const* c
 __global__ __launch_bounds__(256) void paged_compact_kernel(PagedCacheView c, long layer_stride, long scale_layer_stride, int esize, int dim,
                                                             const int* __restrict__ table, long table_stride, int max_pages,
                                                             const int* __restrict__ kept, const int* __restrict__ path, int path_cols,
-                                                            const int* __restrict__ count) {
+                                                            const int* __restrict__ count, int layers) {
     typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
     __shared__ char* column[kCompactPieces];                 // where piece e of token 0 of page 0 lies
     __shared__ long src[2][256], dst[2][256];                // byte offsets of up to 256 moves; [1]: of the scales
     __shared__ int wsum[4];
-    const int b = blockIdx.z, layer = blockIdx.y;
+    const int b = blockIdx.z;
     const int m = min(max(count[b], 0), path_cols), kept_b = kept[b];
     const int per_row = dim * esize / 16;                    // pieces of a (head, token) row
     const int all = 2 * c.heads * per_row, scale_blocks = c.ks ? (2 * c.heads + kCompactPieces - 1) / kCompactPieces : 0;
@@ -490,10 +492,10 @@ __global__ __launch_bounds__(256) void paged_compact_kernel(PagedCacheView c, lo
         const int q = first + e;
         if (scales) {
             const int which = q / c.heads, h = q - which * c.heads;
-            column[e] = reinterpret_cast<char*>((which ? c.vs : c.ks) + layer * scale_layer_stride + (long)h * page);
+            column[e] = reinterpret_cast<char*>((which ? c.vs : c.ks) + (long)h * page);
         } else {
             const int which = q / (c.heads * per_row), rest = q - which * c.heads * per_row, h = rest / per_row;
-            column[e] = static_cast<char*>(which ? c.v : c.k) + (layer * layer_stride + h * c.head_stride) * esize + (rest - h * per_row) * 16;
+            column[e] = static_cast<char*>(which ? c.v : c.k) + h * c.head_stride * esize + (rest - h * per_row) * 16;
         }
     }
     auto page_of = [&](long place) -> int {
@@ -524,8 +526,11 @@ __global__ __launch_bounds__(256) void paged_compact_kernel(PagedCacheView c, lo
         }
         const int moves = wsum[0] + wsum[1] + wsum[2] + wsum[3];
         __syncthreads();
-        if (scales) move_pieces<unsigned>(column, pieces, src[1], dst[1], moves);
-        else move_pieces<u32x4>(column, pieces, src[0], dst[0], moves);
+        // workgroups of a request take the layers in turn: finding the moves is four round trips to memory, once for all of them
+        for (int layer = blockIdx.y; layer < layers; layer += gridDim.y) {
+            if (scales) move_pieces<unsigned>(column, pieces, src[1], dst[1], moves, layer * scale_layer_stride * 4);
+            else move_pieces<u32x4>(column, pieces, src[0], dst[0], moves, layer * layer_stride * esize);
+        }
     }
 }
 
@@ -578,8 +583,13 @@ void launch_paged_compact(const PagedCacheView& c, int layers, long layer_stride
     const int esize = c.ks ? 1 : 2;
     const int blocks = (2 * c.heads * (dim * esize / 16) + kCompactPieces - 1) / kCompactPieces +
                        (c.ks ? (2 * c.heads + kCompactPieces - 1) / kCompactPieces : 0);
-    paged_compact_kernel<<<dim3(blocks, layers, batch), 256, 0, s>>>(c, layer_stride, scale_layer_stride, esize, dim, table, table_stride, max_pages,
-                                                                     kept, path, path_cols, count);
+    // Layers a workgroup takes.  64 requests with trees of 60 nodes, 48 layers, 3 blocks: 8192 workgroups at most (2 layers each)
+    // 55 us, 2048 (5 layers) 63 us; short paths are over before the next workgroup is found: 16 requests with trees of 8, 32
+    // layers, 5 blocks: 7.3 us with 2 layers each, 8.6 with one.
+    const long share = std::max(((long)blocks * batch * layers + 8191) / 8192, (long)(16 + path_cols - 1) / path_cols);
+    const int groups = (int)((layers + share - 1) / share);
+    paged_compact_kernel<<<dim3(blocks, groups, batch), 256, 0, s>>>(c, layer_stride, scale_layer_stride, esize, dim, table, table_stride, max_pages,
+                                                                     kept, path, path_cols, count, layers);
 }
 
 }  // namespace mw
