@@ -224,6 +224,20 @@ int mw_decode_sample(mw_ctx* ctx, int n_audio, int best_of, float temperature, u
                      int32_t* out_ids, int32_t* out_len, float* out_avg_logprob, int32_t* smp_ids, int32_t* smp_len,
                      float* smp_sum_logprob, float* logits_out);
 
+/* Greedy decoding of the last mw_encode(n_audio) with drafted tokens: the ids of mw_decode_greedy in fewer passes over the
+ * decoder (identical up to the rounding of near-equal logits: a pass takes its rows through the same products in other
+ * groupings).  A draft is a transcription of the recording from elsewhere: a smaller model, an earlier pass, the window
+ * before.  Every pass takes a tree of `nodes` tokens per recording: the last token and below it what the drafts propose
+ * next; it yields one token, plus every proposed one that the model would have chosen itself.  A draft is followed from
+ * the place where it agrees with the tokens so far, so it may leave words out or have others; a useless one costs time only.
+ * nodes in 2..64, n_audio * nodes <= max_batch, n_audio <= the context's cache_sequences (mw_fork_cached).
+ * drafts: int32 [n_audio][n_drafts][max_draft] (host memory; ids of text tokens, end-of-text may stand at the end), draft_len
+ * int32 [n_audio][n_drafts]; n_drafts in 0..8, max_draft in 1..1000.  Outputs as mw_decode_greedy; mw_stage_ms[4] is the
+ * number of passes.  Needs ffn_dim >= 3 * d_model.  No counterpart in the reference (decoding stays inside its backend behind
+ * model.transcribe, transcribe.py:123). */
+int mw_decode_drafted(mw_ctx* ctx, int n_audio, int nodes, const int32_t* drafts, const int32_t* draft_len, int n_drafts, int max_draft,
+                      int32_t* out_ids, int32_t* out_len);
+
 /* The uniform in (0, 1) behind the draw of mw_decode_sample for sequence `sequence` (= recording * best_of + sample),
  * sampled position `position` (0 = the first token after the prompt) and token id `token`: host code, no GPU needed.
  * The token drawn at a position is argmax over the unsuppressed ids of logits[id] / temperature - log(-log(u(id))). */

@@ -14,7 +14,7 @@ LIB_PATH = os.environ.get("MW_LIB_PATH") or os.path.join(_HERE, "libmwhip.so")  
 # every symbol include/mwhip.h declares
 SYMBOLS = (
     "mw_create", "mw_fork", "mw_fork_sized", "mw_fork_cached", "mw_set_weight", "mw_finalize", "mw_set_decode_opts", "mw_destroy", "mw_last_error",
-    "mw_logmel", "mw_logmel_noalloc", "mw_encode", "mw_encode_into", "mw_set_encoded", "mw_read_cross_kv", "mw_decode_greedy", "mw_decode_beam", "mw_decode_sample", "mw_sample_uniform", "mw_decode_forced", "mw_transcribe_batch",
+    "mw_logmel", "mw_logmel_noalloc", "mw_encode", "mw_encode_into", "mw_set_encoded", "mw_read_cross_kv", "mw_decode_greedy", "mw_decode_beam", "mw_decode_sample", "mw_decode_drafted", "mw_sample_uniform", "mw_decode_forced", "mw_transcribe_batch",
     "mw_frame_energy_db", "mw_stage_ms", "mw_profile_cross_attention", "mw_profile_decode_gemvs", "mw_set_option", "mw_synchronize",
     "mw_align_frames", "mw_align_create", "mw_align_destroy", "mw_align_last_error", "mw_align_set_weight", "mw_align_finalize",
     "mw_align_emissions", "mw_align_fork", "mw_align_path", "mw_align_segment", "mw_align_segments",
@@ -189,6 +189,7 @@ def load() -> C.CDLL:
     lib.mw_decode_greedy.argtypes = [vp, C.c_int, vp, vp, f32p]
     lib.mw_decode_beam.argtypes = [vp, C.c_int, C.c_int, C.c_float, vp, vp, f32p, vp, vp, f32p]
     lib.mw_decode_sample.argtypes = [vp, C.c_int, C.c_int, C.c_float, C.c_uint32, vp, vp, vp, f32p, vp, vp, f32p, f32p]
+    lib.mw_decode_drafted.argtypes = [vp, C.c_int, C.c_int, vp, vp, C.c_int, C.c_int, vp, vp]
     lib.mw_sample_uniform.argtypes = [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32]
     lib.mw_sample_uniform.restype = C.c_float
     lib.mw_decode_forced.argtypes = [vp, C.c_int, vp, C.c_int, f32p]

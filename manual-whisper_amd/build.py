@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmwhip.so")
 SOURCES = ["engine.hip", "kernels_mel.hip", "kernels_gemm.hip", "kernels_enc.hip", "kernels_dec.hip", "kernels_vad.hip", "kernels_w2v.hip", "aligner.hip",
-           "kernels_paged.hip", "kernels_tree.hip", "paged.hip"]
+           "kernels_paged.hip", "kernels_tree.hip", "kernels_draft.hip", "paged.hip"]
 HEADERS = [os.path.join(CSRC, "mw_kernels.h"), os.path.join(os.path.dirname(HERE), "include", "mwhip.h")]
 ARCH = "gfx950"
 # no packed fp32 instructions: some forms of v_pk_add/mul/fma_f32, which the compiler makes of ordinary float code, have

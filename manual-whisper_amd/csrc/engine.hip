@@ -9,6 +9,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <array>
 #include <map>
 #include <mutex>
 #include <set>
@@ -130,6 +131,13 @@ struct mw_ctx {
     float *sp_sum_lp = nullptr, *sp_part_m = nullptr, *sp_part_s = nullptr, *sp_part_v = nullptr, *sp_part_l = nullptr;
     int* sp_part_i = nullptr;
     uint8_t* sp_active = nullptr;
+
+    // drafted decoding (allocated on first use, for max_batch rows)
+    DraftParams dr{};
+    int *dr_table = nullptr, *dr_row_start = nullptr, *dr_admitted = nullptr, *dr_positions = nullptr, *dr_units = nullptr, *dr_unit_start = nullptr,
+        *dr_best = nullptr, *dr_path = nullptr, *dr_drafts = nullptr, *dr_draft_len = nullptr;
+    long* dr_slots = nullptr; unsigned* dr_mask = nullptr; void* dr_work = nullptr;
+    hipGraph_t dr_graph = nullptr; hipGraphExec_t dr_graph_exec = nullptr; std::array<int, 6> dr_graph_key{};
 
     // decode options
     std::vector<int32_t> prompt;
@@ -415,6 +423,8 @@ extern "C" void mw_destroy(mw_ctx* ctx) {
             if (ctx->graph_exec[i][j]) (void)hipGraphExecDestroy(ctx->graph_exec[i][j]);
             if (ctx->graph[i][j]) (void)hipGraphDestroy(ctx->graph[i][j]);
         }
+    if (ctx->dr_graph_exec) (void)hipGraphExecDestroy(ctx->dr_graph_exec);
+    if (ctx->dr_graph) (void)hipGraphDestroy(ctx->dr_graph);
     for (void* p : ctx->allocs) (void)hipFree(p);
     if (ctx->stage) (void)hipFree(ctx->stage);
     for (auto& e : ctx->ev) if (e) (void)hipEventDestroy(e);
@@ -475,6 +485,8 @@ static int drop_graphs(mw_ctx* ctx) {
             if (ctx->graph_exec[i][j]) { (void)hipGraphExecDestroy(ctx->graph_exec[i][j]); ctx->graph_exec[i][j] = nullptr; }
             if (ctx->graph[i][j]) { (void)hipGraphDestroy(ctx->graph[i][j]); ctx->graph[i][j] = nullptr; }
         }
+    if (ctx->dr_graph_exec) { (void)hipGraphExecDestroy(ctx->dr_graph_exec); ctx->dr_graph_exec = nullptr; }
+    if (ctx->dr_graph) { (void)hipGraphDestroy(ctx->dr_graph); ctx->dr_graph = nullptr; }
     return MW_OK;
 }
 
@@ -973,8 +985,34 @@ static void enqueue_step_tail(mw_ctx* ctx, int B, bool want_logits, const Finali
 // The launches of decoder layer `li` for one position: six weight-streaming projections (GEMVs) and the two
 // attention launches.  `parts`: kLayerGemv, kLayerAttn or both (the measurement entry points time them apart).
 enum { kLayerGemv = 1, kLayerAttn = 2 };
+
+// The self-attention cache of layer `li` as pages of kDraftPage tokens (drafted decoding; the other decodes keep one stretch per
+// sequence in the same memory).
+constexpr int kDraftPage = 64;
+static int draft_pages(const mw_ctx* ctx) { return (int)((long)ctx->max_batch * ctx->d.n_text_ctx / kDraftPage); }
+static PagedCacheView draft_cache(mw_ctx* ctx, int li) {
+    const long layer = (long)ctx->max_batch * ctx->d.d_model * ctx->d.n_text_ctx;
+    return PagedCacheView{ctx->selfK + li * layer, ctx->selfV + li * layer, nullptr, nullptr, (long)ctx->d.n_heads * kDraftPage * kHeadDim,
+                          kDraftPage * kHeadDim, kHeadDim, draft_pages(ctx), 6, ctx->d.n_heads};
+}
+// What the self-attention of a pass over drafted tokens needs besides the layer: rows q|k|v [rows][3D] (q scaled) go into their
+// pages and come back attended over them in `out` [rows][D].
+struct DraftPass { int rows, max_nodes, table_cols; const unsigned* mask; int mask_words; };
+static void draft_self_attention(mw_ctx* ctx, int li, const f16* qkv, f16* out, const DraftPass& dp) {
+    const int D = ctx->d.d_model;
+    const PagedCacheView c = draft_cache(ctx, li);
+    launch_paged_write(c, kHeadDim, 0, qkv + D, qkv + 2 * D, 3L * D, kHeadDim, 3L * D, kHeadDim, ctx->dr_slots, dp.rows, ctx->stream);
+    TreeAttnParams p{};
+    p.c = c; p.dim = kHeadDim; p.heads = ctx->d.n_heads; p.rows = dp.rows; p.batch = ctx->dr.n_audio; p.max_nodes = dp.max_nodes;
+    p.q = qkv; p.q_row = 3L * D; p.q_head = kHeadDim; p.out = out; p.out_row = D; p.out_head = kHeadDim;
+    p.table = ctx->dr_table; p.table_stride = dp.table_cols; p.max_pages = dp.table_cols; p.kept = ctx->dr.kept; p.row_start = ctx->dr_row_start;
+    p.units = ctx->dr_units; p.unit_start = ctx->dr_unit_start; p.n_units = ctx->dr.n_audio;       // short caches: no request is cut
+    p.mask = dp.mask; p.mask_words = dp.mask_words; p.scale = 1.f;
+    launch_tree_attention(p, ctx->stream);
+}
+
 static void enqueue_layer(mw_ctx* ctx, int li, int B, bool want_logits, const FinalizeParams& fp, int max_keys, const BeamParams* beam,
-                          int parts = kLayerGemv | kLayerAttn, const SampleParams* samp = nullptr) {
+                          int parts = kLayerGemv | kLayerAttn, const SampleParams* samp = nullptr, const DraftPass* draft = nullptr) {
     const mw_model_desc& d = ctx->d;
     const int D = d.d_model, F = d.ffn_dim, H = d.n_heads, Tc = d.n_text_ctx;
     hipStream_t s = ctx->stream;
@@ -995,10 +1033,12 @@ static void enqueue_layer(mw_ctx* ctx, int li, int B, bool want_logits, const Fi
     if (gemv) {   // LN1 + QKV; k/v go straight into the cache at the current position
         GemvParams p = base(3 * D, D, l.qkv);
         p.x32 = ctx->dx; p.ln_g = l.ln1.g; p.ln_b = l.ln1.b; p.scale = qscale; p.scale_ncols = D;
-        p.out_mode = GV_QKV; p.out16 = ctx->dq; p.kcache = sk; p.vcache = sv;
+        if (draft) { p.out_mode = GV_F16; p.out16 = ctx->dhid; }          // q | k | v rows (3 D <= ffn_dim)
+        else { p.out_mode = GV_QKV; p.out16 = ctx->dq; p.kcache = sk; p.vcache = sv; }
         launch_gemv(p, s);
     }
-    if (attn) launch_dec_self_attn(ctx->dq, sk, sv, ctx->datt, B, H, Tc, ctx->st, s, beam ? beam->src_rows : nullptr, max_keys);
+    if (draft) draft_self_attention(ctx, li, ctx->dhid, ctx->datt, *draft);
+    else if (attn) launch_dec_self_attn(ctx->dq, sk, sv, ctx->datt, B, H, Tc, ctx->st, s, beam ? beam->src_rows : nullptr, max_keys);
     if (gemv) { GemvParams p = base(D, D, l.out); p.xin16 = ctx->datt; p.out_mode = GV_RESID; p.out32 = ctx->dx; launch_gemv(p, s); }
     if (gemv) {   // LN2 + cross-attention query
         GemvParams p = base(D, D, l.cq);
@@ -1013,6 +1053,8 @@ static void enqueue_layer(mw_ctx* ctx, int li, int B, bool want_logits, const Fi
         if (beam) cross_attention(ctx, li, ctx->dq, ctx->datt, B, beam->beam, 0, (ctx->skip_done && ctx->can_end) ? beam->completed : nullptr, beam->beam);
         // samples: the cache of recording r / best_of, ended flags per sequence
         else if (samp) cross_attention(ctx, li, ctx->dq, ctx->datt, B, samp->best_of, 0, samp->skip_ended ? samp->finished : nullptr, 1);
+        // drafted tokens: the rows of a recording's tree share its cache, read once for all of them
+        else if (draft) cross_attention(ctx, li, ctx->dq, ctx->datt, B, ctx->dr.nodes, 0, (ctx->skip_done && ctx->can_end) ? ctx->dr.finished : nullptr, ctx->dr.nodes);
         else cross_attention(ctx, li, ctx->dq, ctx->datt, B, 1, 0, (ctx->skip_done && ctx->can_end && !want_logits) ? fp.finished : nullptr, 1);
     }
     if (gemv) {
@@ -1051,7 +1093,8 @@ static FinalizeParams finalize_params(mw_ctx* ctx, int n_forced) {
 // Beam search (beam > 1): B recordings, each prompt once; the k/v rows go to the cache rows of the recording's
 // first beam, `src_rows` points every beam at them, and dx gets `beam` copies of each last row.
 // kv_rep > 1 (samples): sequence b reads the cross-attention K/V of recording b / kv_rep.
-static int run_prefill(mw_ctx* ctx, int B, int P, int beam = 1, int* src_rows = nullptr, int kv_rep = 1) {
+// draft (drafted decoding): the rows go into pages and attend over them.
+static int run_prefill(mw_ctx* ctx, int B, int P, int beam = 1, int* src_rows = nullptr, int kv_rep = 1, const DraftPass* draft = nullptr) {
     const mw_model_desc& d = ctx->d;
     const int D = d.d_model, F = d.ffn_dim, H = d.n_heads, Tc = d.n_text_ctx;
     const int M = B * P;
@@ -1070,7 +1113,8 @@ static int run_prefill(mw_ctx* ctx, int B, int P, int beam = 1, int* src_rows = 
         const DecLayerW& l = ctx->dec[li];
         launch_layernorm(ctx->x, l.ln1.g, l.ln1.b, ctx->xn, nullptr, M, D, s);
         {   GemmParams p = gemm(ctx->xn, D, l.qkv, 3 * D); p.scale = qscale; p.scale_ncols = D; p.C = qkv; p.ldc = 3 * D; launch_gemm(p, s); }
-        launch_prefill_self_attn(qkv, ctx->selfK + li * self_layer, ctx->selfV + li * self_layer, ctx->att, B, H, P, Tc, D, s, beam);
+        if (draft) draft_self_attention(ctx, li, qkv, ctx->att, *draft);
+        else launch_prefill_self_attn(qkv, ctx->selfK + li * self_layer, ctx->selfV + li * self_layer, ctx->att, B, H, P, Tc, D, s, beam);
         {   GemmParams p = gemm(ctx->att, D, l.out, D); p.out_mode = OUT_RESID_F32; p.C = ctx->x; p.ldc = D; launch_gemm(p, s); }
         launch_layernorm(ctx->x, l.ln2.g, l.ln2.b, ctx->xn, nullptr, M, D, s);
         {   GemmParams p = gemm(ctx->xn, D, l.cq, D); p.scale = qscale; p.scale_ncols = D; p.C = cq; p.ldc = D; launch_gemm(p, s); }
@@ -1337,6 +1381,158 @@ extern "C" int mw_decode_beam(mw_ctx* ctx, int n_audio, int beam, float patience
                     hyp_ids[((size_t)a * beam + c) * max_new + i] = (have && i < hyps[c].len) ? hyps[c].tok[i] : ctx->eot;
         }
     }
+    return MW_OK;
+}
+
+// Drafted greedy decoding.  The prompt goes through the decoder in one pass whose rows are a chain; every pass after it takes a
+// tree of `nodes` tokens per recording: root = the last token, below it what the drafts propose.  A pass files the root's
+// successor and every drafted token that the model would have chosen itself.
+static PlanParams draft_plan(mw_ctx* ctx, int rows, int table_cols, bool tree) {
+    const DraftParams& r = ctx->dr;
+    PlanParams p{};
+    p.batch = r.n_audio; p.rows = rows; p.page_shift = 6; p.max_pages = table_cols; p.n_pages = r.n_pages;
+    p.kept = r.kept; p.fresh = tree ? r.fresh_tree : r.fresh_prompt; p.parents = tree ? r.parents : nullptr;
+    p.table = ctx->dr_table; p.table_stride = table_cols;
+    p.pages_in = r.pages; p.pages_out = const_cast<int*>(r.pages_after); p.free_list = r.free_list;
+    p.n_free_in = r.n_free; p.n_free_out = const_cast<int*>(r.n_free_after);
+    p.row_start = ctx->dr_row_start; p.admitted = ctx->dr_admitted; p.positions = ctx->dr_positions; p.slots = ctx->dr_slots;
+    p.mask = ctx->dr_mask; p.mask_words = tree ? (r.nodes + 31) / 32 : 0;
+    p.units = ctx->dr_units; p.unit_start = ctx->dr_unit_start; p.chunk_units = 0; p.chunk_min = 64;
+    return p;
+}
+// Final LayerNorm and logits of `rows` rows of dx, acceptance of `trees` (row_start) under `suppress`.
+static void enqueue_draft_tail(mw_ctx* ctx, int rows, const int* row_start, int depth, const uint8_t* suppress) {
+    const mw_model_desc& d = ctx->d;
+    hipStream_t s = ctx->stream;
+    launch_layernorm(ctx->dx, ctx->dec_ln.g, ctx->dec_ln.b, ctx->dxn, nullptr, rows, d.d_model, s);
+    GemvParams g{};
+    g.B = rows; g.N = d.vocab; g.K = d.d_model; g.W = ctx->tok_emb; g.scale = 1.f; g.H = d.n_heads; g.D = d.d_model; g.Tctx = d.n_text_ctx;
+    g.st = ctx->st; g.nv = 16; g.xin16 = ctx->dxn; g.out_mode = GV_LOGITS; g.out32 = ctx->logits;
+    g.mask_first = ctx->mask_first; g.mask_rest = ctx->mask_rest;
+    g.part_val = ctx->part_val; g.part_idx = ctx->part_idx; g.n_parts = ctx->n_parts;
+    launch_gemv(g, s);
+    AcceptParams a{};
+    a.logits = ctx->logits; a.stride = d.vocab; a.dtype = 0; a.rows = rows; a.vocab = d.vocab; a.batch = ctx->dr.n_audio; a.depth = depth;
+    a.suppress = suppress; a.tokens = ctx->dr.tokens; a.parents = ctx->dr.parents; a.row_start = row_start;
+    a.best = ctx->dr_best; a.path = ctx->dr_path; a.count = const_cast<int*>(ctx->dr.count); a.out_tokens = const_cast<int*>(ctx->dr.out_tokens);
+    a.workspace = ctx->dr_work;
+    launch_tree_accept(a, s);
+}
+static void enqueue_draft_step(mw_ctx* ctx, int table_cols) {
+    const mw_model_desc& d = ctx->d;
+    const DraftParams& r = ctx->dr;
+    const int rows = r.n_audio * r.nodes;
+    hipStream_t s = ctx->stream;
+    const DraftPass pass{rows, r.nodes, table_cols, ctx->dr_mask, (r.nodes + 31) / 32};
+    launch_paged_plan(draft_plan(ctx, rows, table_cols, true), s);
+    launch_draft_embed(r.tokens, ctx->dr_positions, ctx->tok_emb, ctx->dec_pos, d.d_model, d.n_text_ctx, ctx->dx, rows, s);
+    const FinalizeParams fp{};
+    for (int li = 0; li < d.dec_layers; ++li) enqueue_layer(ctx, li, rows, false, fp, 0, nullptr, kLayerGemv | kLayerAttn, nullptr, &pass);
+    enqueue_draft_tail(ctx, rows, ctx->dr_row_start, r.nodes, ctx->mask_rest);
+    launch_paged_compact(draft_cache(ctx, 0), d.dec_layers, (long)ctx->max_batch * d.d_model * d.n_text_ctx, 0, kHeadDim, ctx->dr_table, table_cols,
+                         table_cols, r.kept, ctx->dr_path, r.nodes, r.count, r.n_audio, s);
+    launch_draft_step(r, r.nodes, 0, s);
+}
+
+extern "C" int mw_decode_drafted(mw_ctx* ctx, int n_audio, int nodes, const int32_t* drafts, const int32_t* draft_len, int n_drafts, int max_draft,
+                                 int32_t* out_ids, int32_t* out_len) {
+    if (!ctx) return MW_ERR_ARG;
+    if (!ctx->finalized) return fail(ctx, MW_ERR_STATE, "mw_decode_drafted: mw_finalize has not succeeded yet");
+    if (!ctx->opts_set) return fail(ctx, MW_ERR_STATE, "mw_decode_drafted: call mw_set_decode_opts first");
+    const mw_model_desc& d = ctx->d;
+    if (nodes < 2 || nodes > kMaxTreeNodes) return fail(ctx, MW_ERR_ARG, "mw_decode_drafted: nodes must be in 2.." + std::to_string(kMaxTreeNodes));
+    if (n_audio < 1 || (long)n_audio * nodes > ctx->max_batch)
+        return fail(ctx, MW_ERR_ARG, "mw_decode_drafted: n_audio * nodes must be in 1.." + std::to_string(ctx->max_batch) + " (max_batch)");
+    if (n_audio > ctx->cache_seqs) return fail(ctx, MW_ERR_ARG, "mw_decode_drafted: n_audio exceeds the K/V cache (" + std::to_string(ctx->cache_seqs) + " recordings)");
+    if (ctx->enc_batch != n_audio) return fail(ctx, MW_ERR_STATE, "mw_decode_drafted: n_audio differs from the last mw_encode");
+    if (!out_ids || !out_len) return fail(ctx, MW_ERR_ARG, "mw_decode_drafted: null output");
+    if (n_drafts < 0 || n_drafts > kMaxDrafts) return fail(ctx, MW_ERR_ARG, "mw_decode_drafted: n_drafts must be in 0.." + std::to_string(kMaxDrafts));
+    if (n_drafts > 0 && (!drafts || !draft_len || max_draft < 1 || max_draft > 1000)) return fail(ctx, MW_ERR_ARG, "mw_decode_drafted: drafts need ids, lengths and max_draft in 1..1000");
+    if (3 * d.d_model > d.ffn_dim) return fail(ctx, MW_ERR_ARG, "mw_decode_drafted: needs ffn_dim of at least 3 * d_model");
+    const int P = (int)ctx->prompt.size(), max_new = ctx->max_new;
+    const int table_cols = (d.n_text_ctx + nodes + kDraftPage - 1) / kDraftPage;
+    if ((long)n_audio * table_cols > draft_pages(ctx))
+        return fail(ctx, MW_ERR_ARG, "mw_decode_drafted: the self-attention cache has no room for that many trees (raise max_batch)");
+    const size_t n_tok = (size_t)n_audio * n_drafts * max_draft;
+    if (n_drafts > 0) {
+        if (is_device_ptr(drafts) || is_device_ptr(draft_len)) return fail(ctx, MW_ERR_ARG, "mw_decode_drafted: drafts and draft_len must be host memory");
+        for (int i = 0; i < n_audio * n_drafts; ++i) {
+            if (draft_len[i] < 0 || draft_len[i] > max_draft) return fail(ctx, MW_ERR_ARG, "mw_decode_drafted: draft length out of range");
+            for (int j = 0; j < draft_len[i]; ++j)
+                if (drafts[(size_t)i * max_draft + j] < 0 || drafts[(size_t)i * max_draft + j] >= d.vocab)
+                    return fail(ctx, MW_ERR_ARG, "mw_decode_drafted: token id out of range");
+        }
+    }
+    HIPCHK(hipSetDevice(ctx->device));
+    if (!ctx->dr_work) {            // first use: trees of max_batch rows in all, prompts of n_text_ctx rows for half as many recordings
+        const size_t MB = ctx->max_batch, rows = MB * d.n_text_ctx, pages = draft_pages(ctx), cols = d.n_text_ctx / kDraftPage + 3;
+        DraftParams& r = ctx->dr;
+        int *count = nullptr, *out_tokens = nullptr, *pages_after = nullptr, *n_free_after = nullptr;
+        ALLOC(r.kept, MB); ALLOC(r.len, MB); ALLOC(r.shift, MB * kMaxDrafts); ALLOC(r.fresh_prompt, MB); ALLOC(r.fresh_tree, MB); ALLOC(r.first_rows, MB + 1);
+        ALLOC(r.pages, MB); ALLOC(r.n_free, 1); ALLOC(r.free_list, pages); ALLOC(pages_after, MB); ALLOC(n_free_after, 1);
+        ALLOC(r.tokens, MB); ALLOC(r.parents, MB); ALLOC(count, MB); ALLOC(out_tokens, MB);
+        r.pages_after = pages_after; r.n_free_after = n_free_after; r.count = count; r.out_tokens = out_tokens;
+        ALLOC(ctx->dr_table, MB * cols); ALLOC(ctx->dr_row_start, MB + 1); ALLOC(ctx->dr_admitted, MB); ALLOC(ctx->dr_positions, rows);
+        ALLOC(ctx->dr_slots, rows); ALLOC(ctx->dr_mask, MB * (kMaxTreeNodes / 32)); ALLOC(ctx->dr_units, MB * 4); ALLOC(ctx->dr_unit_start, MB + 1);
+        ALLOC(ctx->dr_best, MB); ALLOC(ctx->dr_path, MB); ALLOC(ctx->dr_drafts, MB * kMaxDrafts * 1000); ALLOC(ctx->dr_draft_len, MB * kMaxDrafts);
+        float* work = nullptr;
+        ALLOC(work, MB * kAcceptMaxParts * 2);
+        ctx->dr_work = work;
+    }
+    hipStream_t s = ctx->stream;
+    DraftParams& r = ctx->dr;
+    r.st = ctx->st; r.n_audio = n_audio; r.nodes = nodes; r.n_drafts = n_drafts; r.max_draft = n_drafts > 0 ? max_draft : 1; r.max_new = max_new; r.eot = ctx->eot;
+    r.n_text_ctx = d.n_text_ctx; r.n_pages = draft_pages(ctx); r.drafts = ctx->dr_drafts; r.draft_len = ctx->dr_draft_len;
+    r.out_ids = ctx->out_ids; r.out_len = ctx->out_len; r.finished = ctx->finished;
+    std::vector<int32_t> f((size_t)n_audio * P);
+    for (int b = 0; b < n_audio; ++b) memcpy(&f[(size_t)b * P], ctx->prompt.data(), P * 4);
+    HIPCHK(hipMemcpyAsync(ctx->forced, f.data(), f.size() * 4, hipMemcpyHostToDevice, s));
+    if (n_drafts > 0) {
+        HIPCHK(hipMemcpyAsync(ctx->dr_drafts, drafts, n_tok * 4, hipMemcpyHostToDevice, s));
+        HIPCHK(hipMemcpyAsync(ctx->dr_draft_len, draft_len, (size_t)n_audio * n_drafts * 4, hipMemcpyHostToDevice, s));
+    }
+    HIPCHK(hipStreamSynchronize(s));
+    HIPCHK(hipEventRecord(ctx->ev[3], s));
+    launch_draft_init(r, P, s);
+    launch_paged_plan(draft_plan(ctx, n_audio * P, table_cols, false), s);
+    const DraftPass prompt{n_audio * P, P, table_cols, nullptr, 0};
+    int rc = run_prefill(ctx, n_audio, P, 1, nullptr, 1, &prompt);
+    if (rc) return rc;
+    enqueue_draft_tail(ctx, n_audio, r.first_rows, 1, ctx->mask_first);
+    launch_draft_step(r, 1, P, s);
+    HIPCHK(hipGetLastError());
+    // every pass files one token at least; the arguments of its launches are the same throughout
+    const std::array<int, 6> key{n_audio, nodes, n_drafts, r.max_draft, max_new, ctx->eot};
+    int n_polls = 0, passes = 1;
+    for (int step = 1; step < max_new; ++step, ++passes) {
+        if (ctx->use_graph) {
+            if (!ctx->dr_graph_exec || ctx->dr_graph_key != key) {
+                if (ctx->dr_graph_exec) {
+                    HIPCHK(hipStreamSynchronize(s));
+                    (void)hipGraphExecDestroy(ctx->dr_graph_exec); ctx->dr_graph_exec = nullptr;
+                }
+                if (ctx->dr_graph) { (void)hipGraphDestroy(ctx->dr_graph); ctx->dr_graph = nullptr; }
+                HIPCHK(hipStreamBeginCapture(s, hipStreamCaptureModeThreadLocal));
+                enqueue_draft_step(ctx, table_cols);
+                HIPCHK(hipStreamEndCapture(s, &ctx->dr_graph));
+                HIPCHK(hipGraphInstantiate(&ctx->dr_graph_exec, ctx->dr_graph, nullptr, nullptr, 0));
+                ctx->dr_graph_key = key;
+            }
+            HIPCHK(hipGraphLaunch(ctx->dr_graph_exec, s));
+        } else { enqueue_draft_step(ctx, table_cols); HIPCHK(hipGetLastError()); }
+        if (step % ctx->check_every == 0) {
+            bool all_done = false;
+            rc = poll_finished(ctx, n_polls++, n_audio, &all_done);
+            if (rc) return rc;
+            if (all_done) { ++passes; break; }
+        }
+    }
+    ctx->stage_ms[4] = (float)passes;
+    HIPCHK(hipEventRecord(ctx->ev[4], s));
+    HIPCHK(hipMemcpyAsync(out_ids, ctx->out_ids, (size_t)n_audio * max_new * 4, hipMemcpyDefault, s));
+    HIPCHK(hipMemcpyAsync(out_len, ctx->out_len, (size_t)n_audio * 4, hipMemcpyDefault, s));
+    HIPCHK(hipStreamSynchronize(s));
+    HIPCHK(hipEventElapsedTime(&ctx->stage_ms[3], ctx->ev[3], ctx->ev[4]));
     return MW_OK;
 }
 

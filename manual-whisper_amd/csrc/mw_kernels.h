@@ -344,6 +344,26 @@ struct TreeAttnParams {
     float scale;
     float* workspace;                                          // tree_attn_workspace() bytes; not read when no request is cut
 };
+// Drafted greedy decoding: one context's state.  Trees have `nodes` rows each, so row r belongs to recording r / nodes.
+constexpr int kMaxDrafts = 8, kMaxTreeNodes = 64;              // powers of two; a tree fits one wave
+struct DraftParams {
+    DecState* st;
+    int n_audio, nodes, n_drafts, max_draft, max_new, eot, n_text_ctx, n_pages;
+    const int* drafts; const int* draft_len;    // [n_audio][n_drafts][max_draft], [n_audio][n_drafts]
+    int *kept, *len, *shift;                    // cached tokens, filed tokens [n_audio]; where each draft was followed [n_audio][n_drafts]
+    int *fresh_prompt, *fresh_tree;             // [n_audio]: rows of the prompt's pass and of every other one
+    int *first_rows;                            // [n_audio + 1]: 0, 1, 2, ... (the trees of one row after the prompt)
+    int *pages, *n_free, *free_list;            // as the next plan finds them
+    const int *pages_after, *n_free_after;      // as the last one left them
+    int *tokens, *parents;                      // [n_audio * nodes] the next trees
+    const int *count, *out_tokens;              // of mw_tree_accept
+    int *out_ids, *out_len, *finished;          // [n_audio][max_new], [n_audio], [n_audio]
+};
+void launch_draft_init(const DraftParams& p, int prompt_len, hipStream_t s);
+// depth: columns of out_tokens.  advance: the tokens that are cached now (after the prompt), 0: what was accepted on top.
+void launch_draft_step(const DraftParams& p, int depth, int advance, hipStream_t s);
+void launch_draft_embed(const int* tokens, const int* positions, const f16* tok_emb, const f16* pos_emb, int D, int n_text_ctx, float* x, int rows,
+                        hipStream_t s);
 long tree_attn_workspace(int n_units, int batch, int kv_heads, int group, int max_nodes, int dim);
 void launch_tree_attention(const TreeAttnParams& p, hipStream_t s);
 

@@ -264,6 +264,28 @@ class Engine:
             out += (lg,)
         return out
 
+    def decode_drafted(self, n_audio: int, drafts: Sequence, nodes: int = 8):
+        """Greedy decoding over the last ``encode(n_audio)`` with drafted tokens (``mw_decode_drafted``): -> (ids [n_audio, max_new],
+        lens), those of ``decode_greedy`` up to near-equal logits.  ``drafts``: per recording a list of up to 8 drafts, each a list of
+        token ids.  ``nodes``: tokens a pass takes per recording; ``n_audio * nodes`` sequences must fit ``max_batch``."""
+        if self.opts is None:
+            raise EngineError("set_decode_options first")
+        if len(drafts) != n_audio:
+            raise EngineError(f"drafts must hold one list per recording ({n_audio}), got {len(drafts)}")
+        n_drafts = max((len(d) for d in drafts), default=0)
+        longest = max((len(x) for d in drafts for x in d), default=0)
+        ids = np.empty((n_audio, self.opts.max_new), np.int32)
+        lens = np.empty(n_audio, np.int32)
+        tok = np.zeros((n_audio, max(1, n_drafts), max(1, longest)), np.int32)
+        dl = np.zeros((n_audio, max(1, n_drafts)), np.int32)
+        for b, d in enumerate(drafts):
+            for i, x in enumerate(d):
+                tok[b, i, :len(x)] = x
+                dl[b, i] = len(x)
+        self._check(self._lib.mw_decode_drafted(self._h, n_audio, int(nodes), _ptr(tok), _ptr(dl), n_drafts, tok.shape[2], _ptr(ids), _ptr(lens)),
+                    "mw_decode_drafted")
+        return ids, lens
+
     def transcribe_batch_beam(self, pcm, beam: int, patience: float = 1.0):
         """log-mel -> encoder -> beam search for up to max_batch // beam chunks: -> (ids, lens), as transcribe_batch."""
         n = self._pcm_batch(pcm)
