@@ -125,7 +125,7 @@ static int check_attention(const char* who, const mw_tree_args* a) {
     REFUSE_IF(a->batch < 1 || a->batch > (1 << 20), "batch must be in 1..2^20");
     REFUSE_IF(a->rows < 0 || a->rows > (1 << 30) || a->max_nodes < 0 || a->max_nodes > (1 << 20), "rows must be in 0..2^30 and max_nodes in 0..2^20");
     REFUSE_IF(a->n_units < 0 || a->n_units > (1 << 24), "n_units must be in 0..2^24");
-    REFUSE_IF(a->max_pages < 1 || (int64_t)a->max_pages * a->cache.page_size > INT32_MAX, "max_pages must be at least 1 and a request hold less than 2^31 tokens");
+    REFUSE_IF(a->max_pages < 1 || (int64_t)a->max_pages * a->cache.page_size > INT32_MAX - 4096, "max_pages must be at least 1 and a request hold less than 2^31 tokens");
     REFUSE_IF(a->table_stride < a->max_pages, "table_stride must be at least max_pages");
     REFUSE_IF(a->mask && (a->mask_words < 1 || a->mask_words > (1 << 15) || a->max_nodes > 32 * a->mask_words), "mask_words must hold a bit for every node");
     REFUSE_IF(!(a->scale > 0.f) || isinf(a->scale), "scale must be positive and finite");

@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from typing import Optional
 
 import torch
@@ -28,34 +29,69 @@ from . import _lib
 from .engine import EngineError
 
 _FLOATS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_HALVES = (torch.float16, torch.bfloat16)
 _CODES = (torch.uint8, torch.float8_e4m3fn)
 _E4M3 = 3
 _INT = torch.int32
+
+
+# A call here is a launch of a few microseconds, so the argument structs of include/mwhip.h are packed with `struct` (native
+# alignment, like the compiler's) rather than filled in field by field.
+def _codec(fields):
+    kinds = {C.c_void_p: "P", C.c_int64: "q", C.c_int32: "i", C.c_float: "f"}
+    return "".join(_codec(t._fields_) if hasattr(t, "_fields_") else kinds[t] for _, t in fields)
+
+
+_CACHE = struct.Struct("@" + _codec(_lib.PagedCache._fields_) + "0P")
+_PLAN = struct.Struct("@" + _codec(_lib.PlanArgs._fields_) + "0P")
+_ACCEPT = struct.Struct("@" + _codec(_lib.AcceptArgs._fields_) + "0P")
+_TREE = struct.Struct("@" + _codec(_lib.TreeArgs._fields_) + "0P")
+_calls = None
+
+
+class _Calls:
+    """The entry points with their struct arguments as bytes."""
+
+    def __init__(self):
+        lib = _lib.load()
+        by, i32, i64, vp = C.c_char_p, C.c_int32, C.c_int64, C.c_void_p
+
+        def fn(name, res, *args):
+            return C.CFUNCTYPE(res, *args)((name, lib))
+
+        self.plan = fn("mw_paged_plan", i32, by, i32, vp)
+        self.write = fn("mw_paged_write", i32, by, vp, vp, i32, i64, i64, i64, i64, vp, i64, i32, vp)
+        self.tree_space = fn("mw_tree_attention_workspace", i64, by)
+        self.tree = fn("mw_tree_attention", i32, by, i32, vp)
+        self.accept_space = fn("mw_tree_accept_workspace", i64, by)
+        self.accept = fn("mw_tree_accept", i32, by, i32, vp)
+        self.compact = fn("mw_paged_compact", i32, by, i32, i64, vp, i64, i32, vp, vp, i32, vp, i32, i32, vp)
+
+
+def _c() -> _Calls:
+    global _calls
+    if _calls is None:
+        _calls = _Calls()
+    return _calls
 
 
 def _fail(what: str):
     raise EngineError(what)
 
 
-def _check(rc: int, what: str):
-    if rc != 0:
-        raise EngineError(f"{what} failed ({rc}): {_lib.load().mw_last_error(None).decode()}")
+def _failed(rc: int, what: str):
+    raise EngineError(f"{what} failed ({rc}): {_lib.load().mw_last_error(None).decode()}")
 
 
-def _stream(device: int) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _array(t, name: str, dtype, shape, device: int) -> int:
-    """Address of a contiguous tensor of the expected type, shape (None: any extent) and GPU."""
-    if t.dtype is not dtype or t.dim() != len(shape) or not t.is_contiguous():
-        _fail(f"{name} must be a contiguous {dtype} tensor of {len(shape)} dimensions, got {t.dtype} {tuple(t.shape)}")
-    for have, want in zip(t.shape, shape):
-        if want is not None and have != want:
-            _fail(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    if t.get_device() != device:
-        _fail(f"{name} must be on cuda:{device}, got {t.device}")
-    return t.data_ptr()
+    """Address of a contiguous tensor of the expected type, shape and GPU."""
+    if t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous():
+        return t.data_ptr()
+    _fail(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on cuda:{device}, got {t.dtype} {tuple(t.shape)} "
+          f"strides {t.stride()} on {t.device}")
 
 
 def _gpu_of(t, name: str) -> int:
@@ -64,15 +100,27 @@ def _gpu_of(t, name: str) -> int:
     return t.get_device()
 
 
+def _table(t, device: int):
+    """(address, batch, columns, row stride) of a block table."""
+    if t.dtype is not _INT or t.dim() != 2 or t.get_device() != device:
+        _fail(f"table must be int32 [batch, max_pages] on cuda:{device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    stride, inner = t.stride()
+    batch, columns = t.shape
+    if inner != 1 and columns > 1:
+        _fail(f"table must have dense rows, got strides {t.stride()}")
+    return t.data_ptr(), batch, columns, max(stride, columns)
+
+
 def _rows3(t, name: str, device: int):
     """(address, row stride, head stride) of a [rows, heads, head_dim] tensor whose last dimension is dense."""
-    if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] > 1):
-        _fail(f"{name} must be [rows, heads, head_dim] with dense rows, got {tuple(t.shape)} strides {t.stride()}")
+    if t.dim() != 3 or t.get_device() != device:
+        _fail(f"{name} must be [rows, heads, head_dim] on cuda:{device}, got {tuple(t.shape)} on {t.device}")
     if t.requires_grad:
         _fail(f"{name} requires a gradient, and there is no backward pass")
-    if t.get_device() != device:
-        _fail(f"{name} must be on cuda:{device}, got {t.device}")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+    row, head, inner = t.stride()
+    if inner != 1:
+        _fail(f"{name} must have dense rows, got strides {t.stride()}")
+    return t.data_ptr(), row, head
 
 
 class PagedCache:
@@ -82,30 +130,30 @@ class PagedCache:
     dense and start at multiples of 16 bytes.  ``page_size``: a power of two in 16..4096; ``head_dim``: 64 or 128."""
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
-        if k.dim() not in (4, 5) or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
-            _fail(f"k and v must be [(layers,) pages, heads, page_size, head_dim] of one type and layout, got {tuple(k.shape)} {k.dtype} "
+        shape, strides, dtype = k.shape, k.stride(), k.dtype
+        if len(shape) not in (4, 5) or shape != v.shape or dtype is not v.dtype or strides != v.stride():
+            _fail(f"k and v must be [(layers,) pages, heads, page_size, head_dim] of one type and layout, got {tuple(shape)} {dtype} "
                   f"and {tuple(v.shape)} {v.dtype}")
-        self.device = _gpu_of(k, "k")
-        codes = k.dtype in _CODES
-        if not codes and k.dtype not in (torch.float16, torch.bfloat16):
-            _fail(f"a cache holds float16, bfloat16 or e4m3 codes, got {k.dtype}")
-        if k.stride(-1) != 1 or v.get_device() != self.device:
+        self.device = device = _gpu_of(k, "k")
+        codes = dtype in _CODES
+        if not codes and dtype not in _HALVES:
+            _fail(f"a cache holds float16, bfloat16 or e4m3 codes, got {dtype}")
+        if strides[-1] != 1 or v.get_device() != device:
             _fail("rows of the cache must be dense, and k and v on one GPU")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.layers = k.shape[0] if k.dim() == 5 else None
-        n_pages, heads, page, dim = k.shape[-4:]
-        ks = vs = None
+        self.layers = shape[0] if len(shape) == 5 else None
+        self.n_pages, self.heads, self.page_size, self.head_dim = shape[-4:]
+        ks = vs = 0
         if codes:
             if k_scale is None or v_scale is None:
                 _fail("an e4m3 cache needs its row scales")
-            ks = _array(k_scale, "k_scale", torch.float32, k.shape[:-1], self.device)
-            vs = _array(v_scale, "v_scale", torch.float32, k.shape[:-1], self.device)
+            ks = _array(k_scale, "k_scale", torch.float32, shape[:-1], device)
+            vs = _array(v_scale, "v_scale", torch.float32, shape[:-1], device)
         elif k_scale is not None or v_scale is not None:
             _fail("row scales belong to an e4m3 cache")
-        self.dtype = _E4M3 if codes else _FLOATS[k.dtype]
-        self.page_size, self.heads, self.head_dim, self.n_pages = page, heads, dim, n_pages
-        self.struct = _lib.PagedCache(k.data_ptr(), v.data_ptr(), ks, vs, k.stride(-4), k.stride(-3), k.stride(-2), n_pages, page, heads, dim,
-                                      self.dtype)
+        self.dtype = _E4M3 if codes else _FLOATS[dtype]
+        self._fields = (k.data_ptr(), v.data_ptr(), ks, vs, *strides[-4:-1], self.n_pages, self.page_size, self.heads, self.head_dim, self.dtype)
+        self._bytes = _CACHE.pack(*self._fields)
 
     @classmethod
     def empty(cls, layers: int, n_pages: int, heads: int, page_size: int, head_dim: int, dtype=torch.float16, device="cuda") -> "PagedCache":
@@ -133,43 +181,33 @@ class StepPlan:
     """What ``PagePool.plan`` made: row_start [batch + 1], slots (int64) and positions [rows], mask [rows, words] (None: chains),
     admitted, pages [batch], n_free [1], units [batch + chunks, 4], unit_start [batch + 1]; int32, views of one buffer."""
 
-    _NAMES = ("units", "slots", "row_start", "admitted", "pages", "n_free", "unit_start", "positions", "mask")
-
     def __init__(self, batch: int, rows: int, words: int, n_units: int, device):
-        self.batch, self.rows, self.words, self.n_units = batch, rows, words, n_units
-        self._sizes = (4 * n_units, 2 * rows, batch + 1, batch, batch, 1, batch + 1, rows, rows * words)
-        self._buf = torch.empty(sum(self._sizes), dtype=_INT, device=device)
-        self._parts = None
-
-    def _addresses(self):
-        at, out = self._buf.data_ptr(), []
-        for n in self._sizes:
-            out.append(at)
-            at += 4 * n
-        return out
-
-    def __getattr__(self, name: str):            # the views are made when the first one is asked for
-        if name not in self._NAMES:
-            raise AttributeError(name)
-        if self._parts is None:
-            p = dict(zip(self._NAMES, self._buf.split(self._sizes)))
-            p["units"], p["slots"] = p["units"].view(self.n_units, 4), p["slots"].view(torch.int64)
-            p["mask"] = p["mask"].view(self.rows, self.words) if self.words else None
-            self._parts = p
-        return self._parts[name]
+        sizes = (4 * n_units, 2 * rows, batch + 1, batch, batch, 1, batch + 1, rows, rows * words)
+        buf = torch.empty(4 * n_units + 3 * rows + 4 * batch + 3 + rows * words, dtype=_INT, device=device)
+        units, slots, self.row_start, self.admitted, self.pages, self.n_free, self.unit_start, self.positions, mask = buf.split(sizes)
+        self.units, self.slots = units.view(n_units, 4), slots.view(torch.int64)
+        self.mask = mask.view(rows, words) if words else None
+        at_units = buf.data_ptr()
+        at_slots = at_units + 16 * n_units
+        at_start = at_slots + 8 * rows
+        at_admitted = at_start + 4 * (batch + 1)
+        at_pages = at_admitted + 4 * batch
+        at_free = at_pages + 4 * batch
+        at_first = at_free + 4
+        at_positions = at_first + 4 * (batch + 1)
+        self._at = (at_free, at_start, at_admitted, at_slots, at_positions, at_positions + 4 * rows if words else 0, words, at_units, at_first)
+        self._at_pages = at_pages
 
 
 class PagePool:
     """Tables [batch, max_pages], pages held per request [batch] and the stack of free pages [n_pages] with its height [1]."""
 
     def __init__(self, table, pages, free, n_free, page_size: int):
-        self.device = _gpu_of(table, "table")
-        if table.dim() != 2 or table.dtype is not _INT or table.stride(1) != 1:
-            _fail(f"table must be int32 [batch, max_pages] with dense rows, got {table.dtype} {tuple(table.shape)}")
-        self.batch, self.max_pages = table.shape
-        _array(pages, "pages", _INT, (self.batch,), self.device)
-        _array(free, "free", _INT, (None,), self.device)
-        _array(n_free, "n_free", _INT, (1,), self.device)
+        self.device = device = _gpu_of(table, "table")
+        _, self.batch, self.max_pages, _ = _table(table, device)
+        _array(pages, "pages", _INT, (self.batch,), device)
+        _array(free, "free", _INT, (free.numel(),), device)
+        _array(n_free, "n_free", _INT, (1,), device)
         self.table, self.pages, self.free, self.n_free, self.page_size = table, pages, free, n_free, int(page_size)
 
     @classmethod
@@ -184,18 +222,19 @@ class PagePool:
         32 * ``mask_words`` nodes (default 8 words); None: chains.  ``units``: pieces that the attention's work is cut into
         (0: requests are not cut), none shorter than ``chunk`` keys.  Tables and stack are updated in place; the plan takes
         effect with ``commit``."""
-        dev = self.device
+        dev, batch = self.device, self.batch
         words = 0 if parents is None else 8 if mask_words is None else int(mask_words)
-        if rows < 0 or units < 0 or words < 0:
-            _fail("rows, units and mask_words must not be negative")
-        k, f = _array(kept, "kept", _INT, (self.batch,), dev), _array(fresh, "fresh", _INT, (self.batch,), dev)
-        up = None if parents is None else _array(parents, "parents", _INT, (rows,), dev)
-        p = StepPlan(self.batch, rows, words, self.batch + units, self.table.device)
-        at_units, at_slots, at_start, at_admitted, at_pages, at_free, at_first, at_positions, at_mask = p._addresses()
-        args = _lib.PlanArgs(self.batch, rows, self.page_size, self.free.shape[0], self.max_pages, k, f, up, self.table.data_ptr(),
-                             self.table.stride(0), self.pages.data_ptr(), at_pages, self.free.data_ptr(), self.n_free.data_ptr(), at_free, at_start,
-                             at_admitted, at_slots, at_positions, at_mask if words else None, words, at_units, at_first, units, chunk)
-        _check(_lib.load().mw_paged_plan(C.byref(args), dev, _stream(dev)), "mw_paged_plan")
+        if not (0 <= rows < 1 << 30 and 0 <= units <= 1 << 16 and 1 <= chunk < 1 << 31 and 0 <= words <= 8):
+            _fail(f"rows must be in 0..2^30 - 1, units in 0..65536, chunk positive and mask_words at most 8, got {rows}, {units}, {chunk}, {words}")
+        k, f = _array(kept, "kept", _INT, (batch,), dev), _array(fresh, "fresh", _INT, (batch,), dev)
+        up = 0 if parents is None else _array(parents, "parents", _INT, (rows,), dev)
+        p = StepPlan(batch, rows, words, batch + units, self.table.device)
+        table, _, columns, stride = _table(self.table, dev)
+        args = _PLAN.pack(batch, rows, self.page_size, self.free.shape[0], columns, k, f, up, table, stride, self.pages.data_ptr(), p._at_pages,
+                          self.free.data_ptr(), self.n_free.data_ptr(), *p._at, units, chunk)
+        rc = _c().plan(args, dev, _raw_stream(dev))
+        if rc:
+            _failed(rc, "mw_paged_plan")
         return p
 
     def commit(self, plan: StepPlan) -> None:
@@ -208,14 +247,16 @@ def write(cache: PagedCache, k, v, slots) -> None:
     """Rows ``k``, ``v`` [rows, heads, head_dim] (float16 or bfloat16, any row and head strides) into their ``slots`` (int64
     [rows]; -1 drops a row) of one cache layer (``mw_paged_write``)."""
     dev = cache._one().device
-    rows = k.shape[0] if k.dim() else 0
     pk, k_row, k_head = _rows3(k, "k", dev)
     pv, v_row, v_head = _rows3(v, "v", dev)
-    if tuple(k.shape[1:]) != (cache.heads, cache.head_dim) or v.shape != k.shape or v.dtype is not k.dtype:
+    shape = k.shape
+    rows = shape[0]
+    if shape != (rows, cache.heads, cache.head_dim) or v.shape != shape or v.dtype is not k.dtype:
         _fail(f"k and v must be [rows, {cache.heads}, {cache.head_dim}] of one type, got {tuple(k.shape)} and {tuple(v.shape)}")
-    at = _array(slots, "slots", torch.int64, (rows,), dev)
-    _check(_lib.load().mw_paged_write(C.byref(cache.struct), pk, pv, _FLOATS.get(k.dtype, -1), k_row, k_head, v_row, v_head, at, rows, dev,
-                                      _stream(dev)), "mw_paged_write")
+    rc = _c().write(cache._bytes, pk, pv, _FLOATS.get(k.dtype, -1), k_row, k_head, v_row, v_head,
+                    _array(slots, "slots", torch.int64, (rows,), dev), rows, dev, _raw_stream(dev))
+    if rc:
+        _failed(rc, "mw_paged_write")
 
 
 def tree_attention(q, cache: PagedCache, table, kept, row_start, units, unit_start, max_nodes: int, mask=None, scale: Optional[float] = None,
@@ -226,33 +267,39 @@ def tree_attention(q, cache: PagedCache, table, kept, row_start, units, unit_sta
     dev = cache._one().device
     pq, q_row, q_head = _rows3(q, "q", dev)
     rows, heads, dim = q.shape
-    if dim != cache.head_dim or q.dtype not in (torch.float16, torch.bfloat16):
+    if dim != cache.head_dim or q.dtype not in _HALVES:
         _fail(f"q must be float16 or bfloat16 [rows, heads, {cache.head_dim}], got {q.dtype} {tuple(q.shape)}")
-    if table.dim() != 2 or table.dtype is not _INT or table.stride(1) != 1 or table.get_device() != dev:
-        _fail(f"table must be int32 [batch, max_pages] with dense rows on cuda:{dev}")
-    batch, max_pages = table.shape
+    if not 0 <= max_nodes <= 1 << 20:
+        _fail(f"max_nodes must be in 0..2^20, got {max_nodes}")
+    pt, batch, columns, t_stride = _table(table, dev)
     n_units = units.shape[0]
     if out is None:
         out = torch.empty((rows, heads, dim), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype is not q.dtype:
-        _fail(f"out must be {q.dtype} {tuple(q.shape)}, got {out.dtype} {tuple(out.shape)}")
-    po, o_row, o_head = _rows3(out, "out", dev)
-    pm, words = None, 0
+        po, o_row, o_head = out.data_ptr(), heads * dim, dim
+    else:
+        if out.shape != q.shape or out.dtype is not q.dtype:
+            _fail(f"out must be {q.dtype} {tuple(q.shape)}, got {out.dtype} {tuple(out.shape)}")
+        po, o_row, o_head = _rows3(out, "out", dev)
+    pm = words = 0
     if mask is not None:
         words = mask.shape[1] if mask.dim() == 2 else 0
-        pm = _array(mask, "mask", _INT, (rows, None), dev)
-    args = _lib.TreeArgs(cache.struct, pq, q_row, q_head, po, o_row, o_head, _FLOATS[q.dtype], heads, rows, batch, int(max_nodes), table.data_ptr(),
-                         table.stride(0), max_pages, _array(kept, "kept", _INT, (batch,), dev), _array(row_start, "row_start", _INT, (batch + 1,), dev),
-                         _array(units, "units", _INT, (None, 4), dev), _array(unit_start, "unit_start", _INT, (batch + 1,), dev), n_units, pm, words,
-                         1.0 / math.sqrt(dim) if scale is None else scale, None, 0)
-    lib = _lib.load()
-    need = lib.mw_tree_attention_workspace(C.byref(args))
-    if need < 0:
-        _check(need, "mw_tree_attention")
-    if need:
-        space = torch.empty(need, dtype=torch.uint8, device=q.device)
-        args.workspace, args.workspace_bytes = space.data_ptr(), need
-    _check(lib.mw_tree_attention(C.byref(args), dev, _stream(dev)), "mw_tree_attention")
+        pm = _array(mask, "mask", _INT, (rows, words), dev)
+    fields = cache._fields + (pq, q_row, q_head, po, o_row, o_head, _FLOATS[q.dtype], heads, rows, batch, int(max_nodes), pt, t_stride, columns,
+                              _array(kept, "kept", _INT, (batch,), dev), _array(row_start, "row_start", _INT, (batch + 1,), dev),
+                              _array(units, "units", _INT, (n_units, 4), dev), _array(unit_start, "unit_start", _INT, (batch + 1,), dev), n_units,
+                              pm, words, 1.0 / math.sqrt(dim) if scale is None else scale)
+    c = _c()
+    args = _TREE.pack(*fields, 0, 0)
+    if n_units != batch:                                     # requests may be cut: their pieces' results meet in a workspace
+        need = c.tree_space(args)
+        if need < 0:
+            _failed(need, "mw_tree_attention")
+        if need:
+            space = torch.empty(need, dtype=torch.uint8, device=q.device)
+            args = _TREE.pack(*fields, space.data_ptr(), need)
+    rc = c.tree(args, dev, _raw_stream(dev))
+    if rc:
+        _failed(rc, "mw_tree_attention")
     return out
 
 
@@ -260,42 +307,45 @@ def accept(logits, tokens, parents, row_start, depth: int, suppress=None):
     """Greedy acceptance of the step's trees (``mw_tree_accept``): ``logits`` [rows, vocab] (float32, float16 or bfloat16, any row
     stride), ``tokens``, ``parents`` int32 [rows] -> best [rows], path [batch, depth], count [batch], out_tokens [batch, depth]."""
     dev = _gpu_of(logits, "logits")
-    if logits.dim() != 2 or logits.dtype not in _FLOATS or (logits.stride(1) != 1 and logits.shape[1] > 1):
-        _fail(f"logits must be float [rows, vocab] with dense rows, got {logits.dtype} {tuple(logits.shape)}")
-    if logits.requires_grad:
-        _fail("logits require a gradient, and there is no backward pass")
+    dtype = _FLOATS.get(logits.dtype)
+    if logits.dim() != 2 or dtype is None or logits.requires_grad:
+        _fail(f"logits must be float [rows, vocab] without a gradient, got {logits.dtype} {tuple(logits.shape)}")
     rows, vocab = logits.shape
+    stride, inner = logits.stride()
+    if inner != 1 and vocab > 1:
+        _fail(f"logits must have dense rows, got strides {logits.stride()}")
     batch = row_start.shape[0] - 1 if row_start.dim() == 1 else 0
     depth = int(depth)
-    if batch < 1 or depth < 1:
-        _fail("row_start must have a request at least, and depth be positive")
-    tok, up = _array(tokens, "tokens", _INT, (rows,), dev), _array(parents, "parents", _INT, (rows,), dev)
-    start = _array(row_start, "row_start", _INT, (batch + 1,), dev)
-    sup = None if suppress is None else _array(suppress, "suppress", torch.uint8, (vocab,), dev)
-    lib = _lib.load()
-    args = _lib.AcceptArgs(logits.data_ptr(), logits.stride(0), _FLOATS[logits.dtype], rows, vocab, batch, depth, sup, tok, up, start)
-    need = lib.mw_tree_accept_workspace(C.byref(args))
+    if batch < 1 or not 1 <= depth <= 1024:
+        _fail("row_start must have a request at least, and depth be in 1..1024")
+    head = (logits.data_ptr(), stride, dtype, rows, vocab, batch, depth,
+            0 if suppress is None else _array(suppress, "suppress", torch.uint8, (vocab,), dev), _array(tokens, "tokens", _INT, (rows,), dev),
+            _array(parents, "parents", _INT, (rows,), dev), _array(row_start, "row_start", _INT, (batch + 1,), dev))
+    c = _c()
+    need = c.accept_space(_ACCEPT.pack(*head, 0, 0, 0, 0, 0, 0))
     if need < 0:
-        _check(need, "mw_tree_accept")
+        _failed(need, "mw_tree_accept")
     n = batch * depth
-    buf = torch.empty(rows + 2 * n + batch + need // 4, dtype=_INT, device=logits.device)
+    sizes = (rows, n, batch, n, need // 4)
+    buf = torch.empty(sum(sizes), dtype=_INT, device=logits.device)
     base = buf.data_ptr()
-    args.best, args.path, args.out_tokens, args.count = base, base + 4 * rows, base + 4 * (rows + n), base + 4 * (rows + 2 * n)
-    args.workspace, args.workspace_bytes = base + 4 * (rows + 2 * n + batch), need
-    _check(lib.mw_tree_accept(C.byref(args), dev, _stream(dev)), "mw_tree_accept")
-    return (buf[:rows], buf[rows:rows + n].view(batch, depth), buf[rows + 2 * n:rows + 2 * n + batch],
-            buf[rows + n:rows + 2 * n].view(batch, depth))
+    at_path, at_count = base + 4 * rows, base + 4 * (rows + n)
+    at_tokens = at_count + 4 * batch
+    rc = c.accept(_ACCEPT.pack(*head, base, at_path, at_count, at_tokens, at_tokens + 4 * n, need), dev, _raw_stream(dev))
+    if rc:
+        _failed(rc, "mw_tree_accept")
+    best, path, count, out, _ = buf.split(sizes)
+    return best, path.view(batch, depth), count, out.view(batch, depth)
 
 
 def compact(cache: PagedCache, table, kept, path, count) -> None:
     """Move the accepted rows (``path`` [batch, depth], ``count`` [batch] of ``accept``) to positions kept, kept + 1, ... in every
     layer of ``cache`` (``mw_paged_compact``)."""
     dev = cache.device
-    if table.dim() != 2 or table.dtype is not _INT or table.stride(1) != 1 or table.get_device() != dev:
-        _fail(f"table must be int32 [batch, max_pages] with dense rows on cuda:{dev}")
-    batch, max_pages = table.shape
+    pt, batch, columns, t_stride = _table(table, dev)
     layers, stride = (1, 0) if cache.layers is None else (cache.layers, cache.k.stride(0))
-    columns = path.shape[1] if path.dim() == 2 else 0
-    _check(_lib.load().mw_paged_compact(C.byref(cache.struct), layers, stride, table.data_ptr(), table.stride(0), max_pages,
-                                        _array(kept, "kept", _INT, (batch,), dev), _array(path, "path", _INT, (batch, None), dev), columns,
-                                        _array(count, "count", _INT, (batch,), dev), batch, dev, _stream(dev)), "mw_paged_compact")
+    depth = path.shape[1] if path.dim() == 2 else 0
+    rc = _c().compact(cache._bytes, layers, stride, pt, t_stride, columns, _array(kept, "kept", _INT, (batch,), dev),
+                      _array(path, "path", _INT, (batch, depth), dev), depth, _array(count, "count", _INT, (batch,), dev), batch, dev, _raw_stream(dev))
+    if rc:
+        _failed(rc, "mw_paged_compact")
