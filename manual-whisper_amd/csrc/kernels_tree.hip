@@ -86,13 +86,18 @@ template <int N, int M, int AHEAD, int READS> __device__ __forceinline__ void in
     }
     __builtin_amdgcn_sched_group_barrier(0x008, A * M, 0);
 }
-// 8 e4m3 codes -> 8 values of T (exact)
-template <typename T> __device__ __forceinline__ short8v widen8(unsigned a, unsigned b) {
-    typedef float f2 __attribute__((ext_vector_type(2)));
-    const f2 x0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)a, false), x1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)a, true);
-    const f2 x2 = __builtin_amdgcn_cvt_pk_f32_fp8((int)b, false), x3 = __builtin_amdgcn_cvt_pk_f32_fp8((int)b, true);
-    return short8v{bits_of<T>(x0[0]), bits_of<T>(x0[1]), bits_of<T>(x1[0]), bits_of<T>(x1[1]),
-                   bits_of<T>(x2[0]), bits_of<T>(x2[1]), bits_of<T>(x3[0]), bits_of<T>(x3[1])};
+// 8 e4m3 codes -> 8 values of T (exact, NaN included: two codes an instruction)
+template <typename T> __device__ __forceinline__ u32x4 widen8(unsigned a, unsigned b) {
+    if constexpr (__is_same(T, f16))
+        return u32x4{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, false)),
+                     __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, true)),
+                     __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, false)),
+                     __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, true))};
+    else
+        return u32x4{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, false)),
+                     __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, true)),
+                     __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, false)),
+                     __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, true))};
 }
 
 // LDS of a workgroup: K and V of a tile (at the end: partial results of waves that split the keys), K's and V's row scales.
@@ -180,15 +185,15 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
         for (int i = 0; i < NI; ++i) {
             const int row = 16 * wave + srow + RPL * i;
             if constexpr (KV8) {
-                *reinterpret_cast<short8v*>(&ldsK[k_at<D>(row, 2 * ch)]) = widen8<T>(rk[i][0], rk[i][1]);
-                *reinterpret_cast<short8v*>(&ldsK[k_at<D>(row, 2 * ch + 1)]) = widen8<T>(rk[i][2], rk[i][3]);
+                *reinterpret_cast<u32x4*>(&ldsK[k_at<D>(row, 2 * ch)]) = widen8<T>(rk[i][0], rk[i][1]);
+                *reinterpret_cast<u32x4*>(&ldsK[k_at<D>(row, 2 * ch + 1)]) = widen8<T>(rk[i][2], rk[i][3]);
             } else {
                 *reinterpret_cast<u32x4*>(&ldsK[k_at<D>(row, ch)]) = rk[i];
             }
             u32x4 lo = rv[i], hi = rv[i];
             if constexpr (KV8) {
-                lo = __builtin_bit_cast(u32x4, widen8<T>(rv[i][0], rv[i][1]));
-                hi = __builtin_bit_cast(u32x4, widen8<T>(rv[i][2], rv[i][3]));
+                lo = widen8<T>(rv[i][0], rv[i][1]);
+                hi = widen8<T>(rv[i][2], rv[i][3]);
             }
             if (kv0 + KT > min(kept, key1) || !ok) {                    // (uniform) tiles with rows of this step, or behind the last key
                 // V's infinities and NaN are held back here: in the product they would reach rows that do not see them (0 times
