@@ -367,7 +367,8 @@ typedef struct {
  * requests before it, when it would exceed max_pages, the rows' capacity or (trees) the mask, or when a length is negative;
  * requests that need no new page are admitted whatever the stack holds.  A request without its lengths in range has
  * positions -1 and an empty mask.  Rows behind the last request have slot -1, position -1 and an empty mask.  A parent that
- * is not an earlier node of the same tree counts as none.  kept = fresh = 0 gives everything back.
+ * is not an earlier node of the same tree counts as none.  kept = fresh = 0 gives everything back.  Where the counts claim
+ * more pages than there are, the stack takes back no more than n_pages.
  * The step takes effect with pages_out / n_free_out: planning again from the same counts gives the same plan. */
 int mw_paged_plan(const mw_plan_args* args, int device, void* stream);
 
@@ -386,7 +387,7 @@ typedef struct {
     int32_t n_heads;                      /* query heads: a multiple of the cache's; head h reads K/V head h / (n_heads / cache heads) */
     int32_t rows, batch;
     int32_t max_nodes;                    /* no request has more rows (more are not computed)                           */
-    const int32_t* table; int64_t table_stride; int32_t max_pages;
+    const int32_t* table; int64_t table_stride; int32_t max_pages;          /* max_pages * page_size < 2^31 - 4096       */
     const int32_t* kept; const int32_t* row_start;
     const int32_t* units; const int32_t* unit_start; int32_t n_units;       /* of mw_paged_plan; n_units = batch + chunk_units */
     const uint32_t* mask; int32_t mask_words;                   /* NULL: chains (node i sees nodes 0..i)                 */
@@ -419,8 +420,8 @@ typedef struct {
     void* workspace; int64_t workspace_bytes;       /* mw_tree_accept_workspace() bytes                                  */
 } mw_accept_args;
 
-/* Greedy acceptance: best[r] is the lowest id with the largest logit among those not suppressed (a NaN is never chosen; 0
- * where nothing can be).  From node 0, which is always accepted, the path goes on to the lowest child whose token is the
+/* Greedy acceptance: best[r] is the lowest id with the largest logit among those not suppressed (NaN and minus infinity are
+ * never chosen; 0 where nothing can be).  From node 0, which is always accepted, the path goes on to the lowest child whose token is the
  * arg-max of the node it stands on. */
 int64_t mw_tree_accept_workspace(const mw_accept_args* args);
 int mw_tree_accept(const mw_accept_args* args, int device, void* stream);

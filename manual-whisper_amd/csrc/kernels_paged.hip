@@ -108,7 +108,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
     }
     if (tid == 0) start[B] = (int)total_rows[0];
     block_scan<2>(both, total, ws + 1);
-    const unsigned stack = n_free + total[1];                // pages to be had in this step
+    const unsigned stack = min(n_free + total[1], (unsigned)p.n_pages);      // pages to be had in this step: no more than there are
     unsigned used = 0;                                       // growing requests are admitted up to some point and none behind it
     unsigned long long len_sum = 0;
     int len[kPlanPer];
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
     if (blockIdx.x == 0 && tid == 0) {
         for (int w = 1; w < kPlanWaves; ++w) used = max(used, ws[3][w]);
         p.row_start[B] = start[B];
-        p.n_free_out[0] = (int)min(stack - used, (unsigned)p.n_pages);
+        p.n_free_out[0] = (int)(stack - used);
     }
 
     // page on top of entry `e` of the stack as this step's pushes leave it
@@ -226,8 +226,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
         if (!(state[b] & 2)) continue;
         p.table[(long)b * p.table_stride + held_of[b] + ((int)k - (b ? gend[b - 1] : 0))] = stack_page((int)stack - 1 - (int)k);
     }
-    for (long k = me; k < total[1]; k += threads)
-        if (n_free + k < p.n_pages) p.free_list[n_free + k] = stack_page(n_free + (int)k);
+    for (long k = me; k < (long)stack - n_free; k += threads) p.free_list[n_free + k] = stack_page(n_free + (int)k);
 
     // ---- work units of the attention
     if (p.units && blockIdx.x == gridDim.x - 1) {

@@ -39,6 +39,8 @@ int launched(const char* who, hipError_t e) {
     return MW_ERR_HIP;
 }
 
+constexpr int64_t kMaxThreads = (1LL << 32) - 256;           // of a launch along one dimension
+
 bool misaligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
 
 int check_cache(const char* who, const mw_paged_cache* c) {
@@ -107,7 +109,7 @@ extern "C" int mw_paged_write(const mw_paged_cache* cache, const void* k, const 
     REFUSE_IF(!k || !v || !slots, "null array");
     REFUSE_IF(misaligned(k, 16) || misaligned(v, 16) || k_row_stride % 8 || k_head_stride % 8 || v_row_stride % 8 || v_head_stride % 8,
               "rows must start at multiples of 16 bytes");
-    REFUSE_IF(rows * cache->n_heads * (cache->head_dim / 8) / 256 >= INT32_MAX, "too many rows for one launch");
+    REFUSE_IF(rows * cache->n_heads * (cache->head_dim / 8) > kMaxThreads, "too many rows for one launch");
     OnDevice on(device);
     if (on.err != hipSuccess) return launched(who, on.err);
     launch_paged_write(view_of(*cache), cache->head_dim, dtype == MW_BF16, k, v, k_row_stride, k_head_stride, v_row_stride, v_head_stride,
@@ -125,7 +127,7 @@ static int check_attention(const char* who, const mw_tree_args* a) {
     REFUSE_IF(a->batch < 1 || a->batch > (1 << 20), "batch must be in 1..2^20");
     REFUSE_IF(a->rows < 0 || a->rows > (1 << 30) || a->max_nodes < 0 || a->max_nodes > (1 << 20), "rows must be in 0..2^30 and max_nodes in 0..2^20");
     REFUSE_IF(a->n_units < 0 || a->n_units > (1 << 24), "n_units must be in 0..2^24");
-    REFUSE_IF(a->max_pages < 1 || (int64_t)a->max_pages * a->cache.page_size > INT32_MAX - 4096, "max_pages must be at least 1 and a request hold less than 2^31 tokens");
+    REFUSE_IF(a->max_pages < 1 || (int64_t)a->max_pages * a->cache.page_size > INT32_MAX - 4096, "max_pages must be at least 1 and a request hold less than 2^31 - 4096 tokens");
     REFUSE_IF(a->table_stride < a->max_pages, "table_stride must be at least max_pages");
     REFUSE_IF(a->mask && (a->mask_words < 1 || a->mask_words > (1 << 15) || a->max_nodes > 32 * a->mask_words), "mask_words must hold a bit for every node");
     REFUSE_IF(!(a->scale > 0.f) || isinf(a->scale), "scale must be positive and finite");
@@ -151,8 +153,8 @@ extern "C" int mw_tree_attention(const mw_tree_args* a, int device, void* stream
     const int64_t need = tree_attn_workspace(a->n_units, a->batch, a->cache.n_heads, group, a->max_nodes, a->cache.head_dim);
     REFUSE_IF(need && (!a->workspace || a->workspace_bytes < need || misaligned(a->workspace, 16)),
               "the workspace is smaller than mw_tree_attention_workspace() or not 16-byte aligned");
-    REFUSE_IF(((int64_t)a->n_units * a->cache.n_heads + 8) * (((int64_t)a->max_nodes * group + 127) / 128 + 1) >= INT32_MAX ||
-              (int64_t)a->batch * a->max_nodes * a->n_heads >= INT32_MAX, "too many units or rows for one launch");
+    REFUSE_IF(((int64_t)a->n_units * a->cache.n_heads + 8) * (((int64_t)a->max_nodes * group + 127) / 128) > kMaxThreads / 256 ||
+              (need && (int64_t)a->batch * a->max_nodes * a->n_heads * (a->cache.head_dim / 4) > kMaxThreads), "too many units or rows for one launch");
     OnDevice on(device);
     if (on.err != hipSuccess) return launched(who, on.err);
     TreeAttnParams p{};
@@ -168,7 +170,7 @@ extern "C" int mw_tree_attention(const mw_tree_args* a, int device, void* stream
 static int check_accept(const char* who, const mw_accept_args* a) {
     REFUSE_IF(!a, "null argument");
     REFUSE_IF(a->dtype != MW_F32 && a->dtype != MW_F16 && a->dtype != MW_BF16, "logits must be MW_F32, MW_F16 or MW_BF16");
-    REFUSE_IF(a->rows < 0 || a->rows > (1 << 24), "rows must be in 0..2^24");
+    REFUSE_IF(a->rows < 0 || a->rows >= (1 << 24), "rows must be in 0..2^24 - 1");
     REFUSE_IF(a->vocab < 1 || a->vocab > (1 << 24), "vocab must be in 1..2^24");
     REFUSE_IF(a->batch < 1 || a->batch > (1 << 20), "batch must be in 1..2^20");
     REFUSE_IF(a->depth < 1 || a->depth > kAcceptMaxNodes, "depth must be in 1.." + std::to_string(kAcceptMaxNodes));

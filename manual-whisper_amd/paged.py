@@ -106,9 +106,9 @@ def _table(t, device: int):
         _fail(f"table must be int32 [batch, max_pages] on cuda:{device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     stride, inner = t.stride()
     batch, columns = t.shape
-    if inner != 1 and columns > 1:
-        _fail(f"table must have dense rows, got strides {t.stride()}")
-    return t.data_ptr(), batch, columns, max(stride, columns)
+    if (inner != 1 and columns > 1) or (stride < columns and batch > 1):
+        _fail(f"table must have dense rows of its own, got strides {t.stride()}")
+    return t.data_ptr(), batch, columns, stride if batch > 1 else columns        # (the stride of a dimension of one may be anything)
 
 
 def _rows3(t, name: str, device: int):
@@ -120,7 +120,12 @@ def _rows3(t, name: str, device: int):
     row, head, inner = t.stride()
     if inner != 1:
         _fail(f"{name} must have dense rows, got strides {t.stride()}")
-    return t.data_ptr(), row, head
+    rows, heads, dim = t.shape
+    return t.data_ptr(), row if rows > 1 else 0, head if heads > 1 else dim
+
+
+def _tight(shape, strides):
+    return tuple(shape[-1] if n == 1 else s for n, s in zip(shape[:-1], strides)) + strides[-1:]
 
 
 class PagedCache:
@@ -131,7 +136,11 @@ class PagedCache:
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         shape, strides, dtype = k.shape, k.stride(), k.dtype
-        if len(shape) not in (4, 5) or shape != v.shape or dtype is not v.dtype or strides != v.stride():
+        if 1 in shape[-4:-2] and shape == v.shape:           # the stride of a dimension of one may be anything: the next one's, then
+            strides, other = _tight(shape, strides), _tight(shape, v.stride())
+        else:
+            other = v.stride()
+        if len(shape) not in (4, 5) or shape != v.shape or dtype is not v.dtype or strides != other:
             _fail(f"k and v must be [(layers,) pages, heads, page_size, head_dim] of one type and layout, got {tuple(shape)} {dtype} "
                   f"and {tuple(v.shape)} {v.dtype}")
         self.device = device = _gpu_of(k, "k")
@@ -184,7 +193,7 @@ class StepPlan:
     def __init__(self, batch: int, rows: int, words: int, n_units: int, device):
         sizes = (4 * n_units, 2 * rows, batch + 1, batch, batch, 1, batch + 1, rows, rows * words)
         buf = torch.empty(4 * n_units + 3 * rows + 4 * batch + 3 + rows * words, dtype=_INT, device=device)
-        units, slots, self.row_start, self.admitted, self.pages, self.n_free, self.unit_start, self.positions, mask = buf.split(sizes)
+        units, slots, self.row_start, self.admitted, self.pages, self.n_free, self.unit_start, self.positions, mask = buf.split_with_sizes(sizes)
         self.units, self.slots = units.view(n_units, 4), slots.view(torch.int64)
         self.mask = mask.view(rows, words) if words else None
         at_units = buf.data_ptr()
@@ -245,7 +254,7 @@ class PagePool:
 
 def write(cache: PagedCache, k, v, slots) -> None:
     """Rows ``k``, ``v`` [rows, heads, head_dim] (float16 or bfloat16, any row and head strides) into their ``slots`` (int64
-    [rows]; -1 drops a row) of one cache layer (``mw_paged_write``)."""
+    [rows], all different; -1 drops a row) of one cache layer (``mw_paged_write``)."""
     dev = cache._one().device
     pk, k_row, k_head = _rows3(k, "k", dev)
     pv, v_row, v_head = _rows3(v, "v", dev)
@@ -334,7 +343,7 @@ def accept(logits, tokens, parents, row_start, depth: int, suppress=None):
     rc = c.accept(_ACCEPT.pack(*head, base, at_path, at_count, at_tokens, at_tokens + 4 * n, need), dev, _raw_stream(dev))
     if rc:
         _failed(rc, "mw_tree_accept")
-    best, path, count, out, _ = buf.split(sizes)
+    best, path, count, out, _ = buf.split_with_sizes(sizes)
     return best, path.view(batch, depth), count, out.view(batch, depth)
 
 

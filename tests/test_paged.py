@@ -123,6 +123,18 @@ def test_tensors_are_checked_before_the_library_sees_them():
             fault()
 
 
+def test_calls_beyond_one_launch_are_refused():
+    """A launch has fewer than 2^32 threads along a dimension: what would need more is refused, at the first size that does."""
+    lib = _lib.load()
+    rows = 2 ** 32 // (20 * 8)                                # 8 threads per (row, head) of 64 values
+    assert "too many rows" in _refused(lib.mw_paged_write(C.byref(_cache()), BAD, BAD, 1, 1280, 64, 1280, 64, BAD, rows, 0, None), "mw_paged_write")
+    for fault in (dict(n_units=838861), dict(batch=1 << 13, n_units=(1 << 13) + 1, max_nodes=1 << 11)):          # attention; join of the pieces
+        args = _tree_args(workspace=BAD, workspace_bytes=1 << 62, **fault)
+        assert "too many units or rows" in _refused(lib.mw_tree_attention(C.byref(args), 0, None), "mw_tree_attention")
+    a = _lib.AcceptArgs(BAD, 100, 0, 1 << 24, 100, 2, 4, None, BAD, BAD, BAD, BAD, BAD, BAD, BAD, BAD, 1 << 40)
+    assert "rows" in _refused(lib.mw_tree_accept(C.byref(a), 0, None), "mw_tree_accept")
+
+
 def test_units_of_the_restatement_cover_every_key_once():
     """The oracle's own work units: pieces of a request follow each other and reach its end, whatever the lengths."""
     rng = np.random.default_rng(5)
@@ -242,6 +254,22 @@ def test_plan_of_many_requests_grows_shrinks_and_ends_empty():
         pool.commit(got)
         kept = np.where(np.array(want["admitted"]) == 1, kept + rng.integers(0, 2, B) * fresh, kept)
     assert pool.n_free.item() == 9000 and sorted(pool.free.cpu().tolist()) == list(range(9000))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_free", [0, 3, 4])
+def test_plan_takes_no_more_pages_back_than_there_are(n_free):
+    """Counts that claim 16 pages of a pool of 4: the stack ends at 4, and what grows is served from those."""
+    from manual_whisper_amd import paged
+    table = [[0] * 8, [1] * 8, [-1] * 8]
+    pool = paged.PagePool(_dev(table), _dev([8, 8, 0]), _dev([3, 2, 2, 2]), _dev([n_free]), 16)
+    got = pool.plan(_dev([0, 0, 40]), _dev([0, 0, 8]), 8, units=2, chunk=64)
+    assert got.admitted.cpu().tolist() == [1, 1, 1] and got.pages.cpu().tolist() == [0, 0, 3] and got.n_free.item() == 1
+    stack = ([3, 2, 2, 2][:n_free] + [0] * 8)[:4]
+    assert pool.free.cpu().tolist() == stack and pool.table.cpu().tolist()[2][:3] == stack[:0:-1]
+    assert got.slots.cpu().tolist() == [16 * stack[1] + 8 + i for i in range(8)]
+    none = pool.plan(_dev([0, 0, 60]), _dev([0, 0, 8]), 8)
+    assert none.admitted.cpu().tolist() == [1, 1, 0] and none.pages.cpu().tolist() == [0, 0, 0] and none.n_free.item() == 4
 
 
 def _new_cache(rng, kind, shape, layout="head"):
@@ -628,6 +656,32 @@ def test_compact(kind, layers, heads, dim, page, layout):
     paged.compact(cache, _dev(table), _dev(kept), _dev(path), _dev(count))
     want = ref.compact(before[None] if layers is None else before, table, page, kept, path, count)
     assert (_values(cache, "k") == (want[0] if layers is None else want)).all()
+
+
+@pytest.mark.gpu
+def test_strides_of_dimensions_of_one_and_of_shared_rows():
+    """The stride of a dimension of one says nothing and may be anything; a table whose rows share memory is refused."""
+    from manual_whisper_amd import paged
+    from manual_whisper_amd.engine import EngineError
+    mem = [torch.zeros(3 * 64 * 64, device="cuda", dtype=torch.float16) for _ in range(4)]
+    plain = paged.PagedCache(mem[0].view(3, 1, 64, 64), mem[1].view(3, 1, 64, 64))
+    odd = paged.PagedCache(mem[2].as_strided((3, 1, 64, 64), (4096, 3, 64, 1)), mem[3].as_strided((3, 1, 64, 64), (4096, 0, 64, 1)))
+    rows = torch.randn(1, 64, device="cuda", dtype=torch.float16)
+    slots = torch.tensor([70], device="cuda")
+    paged.write(plain, rows.view(1, 1, 64), rows.view(1, 1, 64), slots)
+    paged.write(odd, rows.as_strided((1, 1, 64), (7, 5, 1)), rows.as_strided((1, 1, 64), (1, 3, 1)), slots)
+    assert mem[0].any() and torch.equal(mem[0], mem[2]) and torch.equal(mem[1], mem[3])
+    table, kept, path = _dev([[1, 0, 2]]), _dev([2]), _dev([[0, 4]])
+    for cache in (plain, odd):
+        paged.compact(cache, table.as_strided((1, 3), (1, 1)), kept, path, _dev([2]))
+    assert mem[0].view(3, 64, 64)[1, 3].any() and torch.equal(mem[0], mem[2])
+    out = [paged.tree_attention(q, cache, table, kept, _dev([0, 1]), _dev([[0, 0, 3, 1]]), _dev([0, 1]), 1)
+           for q, cache in ((rows.view(1, 1, 64), plain), (rows.as_strided((1, 1, 64), (9, 9, 1)), odd))]
+    assert torch.equal(*out)
+    for fault in (lambda: paged.compact(plain, table.expand(2, 3), _dev([2, 2]), _dev([[0, 4]] * 2), _dev([2, 2])),
+                  lambda: paged.PagePool(table.expand(2, 3), _dev([1, 1]), _dev([0]), _dev([0]), 64)):
+        with pytest.raises(EngineError):
+            fault()
 
 
 def _dense_step(q, k, v, ctx, see):
