@@ -16,6 +16,8 @@
 // second launch joins them.
 #include "mw_kernels.h"
 
+#include <type_traits>
+
 namespace mw {
 
 namespace {
@@ -28,7 +30,7 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int KT = 64;                                       // keys of a tile
-constexpr float kGap = 6.f;
+constexpr float kGap = 6.f;                                  // positive: gap > 0 says that a column has seen a key
 
 template <typename T> struct Mat;
 template <> struct Mat<f16> {
@@ -62,6 +64,13 @@ template <typename T> __device__ __forceinline__ u32x4 finite_only(u32x4 u, bool
 }
 template <typename T> __device__ __forceinline__ short bits_of(float x) { return __builtin_bit_cast(short, (T)x); }       // nearest even
 
+// largest of three, NaN passed over (of values that vector instructions made; written out, since the compiler first copies every
+// operand to quiet a NaN)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 __device__ __forceinline__ float column_max(float v) {       // over the four lanes that share a query column
     v = fmaxf(v, __shfl_xor(v, 16));
     return fmaxf(v, __shfl_xor(v, 32));
@@ -141,7 +150,6 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
         for (int s = 0; s < D / 32; ++s) qf[qs][s] = *reinterpret_cast<const short8v*>(src + s * 32 + fg * 8);
     }
     const float to_log2 = p.scale * kLog2e;                  // exponents of two: weight = exp2((s - max) * scale * log2 e)
-    const float by = KV8 ? 1.f : to_log2;                    // what is left to multiply a score by
 
     // ---- staging.  Wave w moves keys 16 w .. 16 w + 15 of a tile: one run of 16, so one page, whose address is scalar.  A lane
     // adds offsets that are the same for every tile.
@@ -221,9 +229,10 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int qs = 0; qs < QT; ++qs) o[d][qs] = float4v{0, 0, 0, 0};
-    float m[QT], l[QT];
+    // a column's weights are 2^(s - ref); `gap`: what an exponent may reach before ref rises (-inf: no key seen yet)
+    float ref[QT], gap[QT], l[QT];
 #pragma unroll
-    for (int qs = 0; qs < QT; ++qs) { m[qs] = -INFINITY; l[qs] = 0.f; }
+    for (int qs = 0; qs < QT; ++qs) { ref[qs] = 0.f; gap[qs] = -INFINITY; l[qs] = 0.f; }
     // e4m3: weights are p_j times V's row scale relative to a power of two above every scale seen so far, so that they stay
     // within fp16's range whatever the scales are; the accumulators are multiplied by it at the end
     float vref = 0.f;
@@ -283,15 +292,15 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
         // ---- the keys that a column does not see
         const int4 there = *reinterpret_cast<const int4*>(lds.page_ok);
         const bool edge = kv0 + KT > kept || kv0 + KT > key1 || !(there.x && there.y && there.z && there.w);
-        if constexpr (KV8) {                                 // K's row scales (already times scale * log2 e)
+        // ---- exponents of the weights: score * scale * log2 e (e4m3: times K's row scale) - ref
 #pragma unroll
-            for (int i = 0; i < NK; ++i) {
-                const float4v s4 = *reinterpret_cast<const float4v*>(&lds.scales[0][(wk * NK + i) * 16 + 4 * fg]);
+        for (int i = 0; i < NK; ++i) {
+            float4v by = float4v{to_log2, to_log2, to_log2, to_log2};
+            if constexpr (KV8) by = *reinterpret_cast<const float4v*>(&lds.scales[0][(wk * NK + i) * 16 + 4 * fg]);      // (all of it)
 #pragma unroll
-                for (int qs = 0; qs < QT; ++qs)
+            for (int qs = 0; qs < QT; ++qs)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) sc[i][qs][r] *= s4[r];
-            }
+                for (int r = 0; r < 4; ++r) sc[i][qs][r] = fmaf(sc[i][qs][r], by[r], -ref[qs]);
         }
         if (edge) {
             const int first = kv0 - kept, limit = key1 - kv0;                 // node of the tile's first key (may be negative)
@@ -310,16 +319,16 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
                         if (!(sees >> ((wk * NK + i) * 16 + 4 * fg + r) & 1)) sc[i][qs][r] = -INFINITY;
             }
         }
-        // ---- online softmax.  m is the reference of a column's weights, 2^(s - m): it rises only when a score exceeds it by more
-        // than kGap, so that weights stay below 2^kGap and the lanes of a column need not agree on a maximum in every tile.
+        // ---- online softmax.  A column's reference rises only when an exponent exceeds kGap, so that weights stay below 2^kGap
+        // and the lanes of a column need not agree on a maximum in every tile.
         bool lift = false;
         float top[QT];
 #pragma unroll
         for (int qs = 0; qs < QT; ++qs) {
             top[qs] = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < NK; ++i) top[qs] = fmaxf(top[qs], fmaxf(fmaxf(sc[i][qs][0], sc[i][qs][1]), fmaxf(sc[i][qs][2], sc[i][qs][3])));
-            lift = lift || top[qs] * by > m[qs] + kGap;
+            for (int i = 0; i < NK; ++i) top[qs] = max3(max3(top[qs], sc[i][qs][0], sc[i][qs][1]), sc[i][qs][2], sc[i][qs][3]);
+            lift = lift || top[qs] > gap[qs];
         }
         float big = 0.f;                                     // e4m3: V's largest row scale in this tile, the same in all lanes
         if constexpr (KV8) {
@@ -339,33 +348,43 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
             }
 #pragma unroll
             for (int qs = 0; qs < QT; ++qs) {
-                const float mn = fmaxf(m[qs], column_max(top[qs]) * by);
-                const float alpha = mn > m[qs] ? __builtin_amdgcn_exp2f(m[qs] - mn) : 1.f;
-                m[qs] = mn;
+                const float up = column_max(top[qs]);
+                const float to = ref[qs] + (gap[qs] > 0.f ? fmaxf(up, 0.f) : up == -INFINITY ? 0.f : up), d = to - ref[qs];
+                const float alpha = gap[qs] > 0.f ? __builtin_amdgcn_exp2f(-d) : 1.f;
+                if (up > -INFINITY) gap[qs] = kGap;
+                ref[qs] = to;
+#pragma unroll
+                for (int i = 0; i < NK; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) sc[i][qs][r] -= d;
                 l[qs] *= alpha;
 #pragma unroll
                 for (int d = 0; d < ND; ++d) { o[d][qs][0] *= alpha * f; o[d][qs][1] *= alpha * f; o[d][qs][2] *= alpha * f; o[d][qs][3] *= alpha * f; }
             }
         }
-        const float vinv = KV8 && vref > 0.f ? 1.f / vref : 0.f;
-#pragma unroll
-        for (int qs = 0; qs < QT; ++qs) {
-            const float ref = m[qs] == -INFINITY ? 0.f : m[qs];               // nothing seen yet: every weight is 0
-            float sum = 0.f;
+        const float vinv = KV8 && vref > 0.f ? 1.f / vref : 0.f;              // (a power of two)
+        auto weigh = [&](auto some_unseen) {
 #pragma unroll
             for (int i = 0; i < NK; ++i) {
                 float4v vs4 = float4v{1, 1, 1, 1};
-                if constexpr (KV8) vs4 = *reinterpret_cast<const float4v*>(&lds.scales[1][(wk * NK + i) * 16 + 4 * fg]);
+                if constexpr (KV8) {
+                    vs4 = *reinterpret_cast<const float4v*>(&lds.scales[1][(wk * NK + i) * 16 + 4 * fg]);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float e = __builtin_amdgcn_exp2f(KV8 ? sc[i][qs][r] - ref : fmaf(sc[i][qs][r], to_log2, -ref));
-                    sum += e;
-                    if constexpr (KV8) sc[i][qs][r] = edge && e == 0.f ? 0.f : e * (vs4[r] * vinv);
-                    else sc[i][qs][r] = e;
+                    for (int r = 0; r < 4; ++r) vs4[r] *= vinv;
                 }
+#pragma unroll
+                for (int qs = 0; qs < QT; ++qs)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float e = __builtin_amdgcn_exp2f(sc[i][qs][r]);
+                        l[qs] += e;                          // of this lane's keys; the column's sum is formed at the end
+                        if constexpr (!KV8) sc[i][qs][r] = e;
+                        else sc[i][qs][r] = decltype(some_unseen)::value && e == 0.f ? 0.f : e * vs4[r];       // whatever the scale of an unseen key
+                    }
             }
-            l[qs] += sum;                                    // of this lane's keys; the column's sum is formed at the end
-        }
+        };
+        if (KV8 && edge) weigh(std::true_type{});
+        else weigh(std::false_type{});
         __builtin_amdgcn_sched_barrier(0);
         // ---- O^T += V^T P^T.  The weights are rounded once to T (half a step of T each, as the result is); the sum above is of
         // the unrounded ones.
@@ -411,6 +430,9 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
     }
 
     // ---- join the waves that split the keys, then normalise and store, or leave the partial result to the second launch
+    float m[QT];                                             // the references, -inf for columns that saw nothing
+#pragma unroll
+    for (int qs = 0; qs < QT; ++qs) m[qs] = gap[qs] > 0.f ? ref[qs] : -INFINITY;
 #pragma unroll
     for (int qs = 0; qs < QT; ++qs) {
         l[qs] = column_sum(l[qs]);
