@@ -566,10 +566,11 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeAttnParams p
 
 // Rows of requests that were cut: the units' partial results, weighted by their maxima.  D / 4 lanes hold a (row, query head),
 // four head dims each.  SHARE: a workgroup per pair whose groups of lanes take the units in turn and are joined through LDS;
-// else every group has a pair of its own.  Eight loads ahead.
+// else every group has a pair of its own.  Bound by the bytes of the partial results (62 MB of wide trees in 14.2 us, 63 MB of
+// chains in 15.0: 4.3 TB/s); four loads ahead of a group that is alone with its pair (eight: 16.1 and 15.3 us), eight of one that shares.
 template <typename T, int D, bool SHARE>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeAttnParams p, int group) {
-    constexpr int LANES = D / 4, GROUPS = 256 / LANES, AHEAD = 8, STEP = SHARE ? GROUPS : 1;
+    constexpr int LANES = D / 4, GROUPS = 256 / LANES, AHEAD = SHARE ? 8 : 4, STEP = SHARE ? GROUPS : 1;
     __shared__ float red_m[GROUPS], red_l[GROUPS];
     __shared__ __attribute__((aligned(16))) float red_o[SHARE ? GROUPS : 1][D];
     const int mine = threadIdx.x / LANES, d = (threadIdx.x % LANES) * 4;
@@ -601,7 +602,8 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeAttnParams p, int gr
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a) {
             const long slot = first + min(u + a * STEP, n - 1) * step;
-            um[a] = ml[slot * 2]; ul[a] = ml[slot * 2 + 1];
+            const float2 two = *reinterpret_cast<const float2*>(ml + slot * 2);
+            um[a] = two.x; ul[a] = two.y;
             x[a] = *reinterpret_cast<const float4v*>(po + slot * D + d);
         }
 #pragma unroll
