@@ -5,15 +5,24 @@
 // bit is set in the row's mask, or without a mask the nodes up to itself.  A row that sees nothing is zero.
 //
 // Bound: the K/V rows of a request are read once per K/V head for all nodes and all query heads of its group, so a step with
-// few columns (nodes x heads per K/V head) is bound by HBM, one with some hundred of them by the matrix cores.
+// few columns (nodes x heads per K/V head) is bound by HBM.  With some hundred columns the matrix products, the exponents and the
+// LDS reads of a tile each come near the time that its rows take to arrive, and none of them alone sets the pace.
 //
 // One workgroup takes one work unit (a stretch of a request's keys), one K/V head and up to 128 query columns.  Keys are on
 // the row index of the matrix instructions, so that a lane's scores belong to one query column: S^T = K Q^T, then
 // O^T = V^T P^T with P straight from the registers of S (its 4-key groups are the k-slots of the second product) and
 // V^T by transposing LDS reads.  Tiles of 64 keys go global -> registers -> LDS, the next tile's loads in flight behind the
-// current tile's products.  The softmax is online: one running maximum and sum per column.
+// current tile's products.  The softmax is online: one running reference and sum per column.
 // A request that is cut into several units leaves its partial results (fp32, with maximum and sum) in the workspace and a
 // second launch joins them.
+//
+// Measured (rows; K/V heads x head_dim; K/V read; this kernel, then the join):
+//   8 requests of 1 row, 207 k tokens of 8 x 128 bf16, 32 heads       849 MB   130 us (6.5 TB/s)                5.2 us
+//   16 trees of 8, 2.5 k tokens of 20 x 64 fp16, 20 heads              13 MB   8.9 us (latency: seven tiles)     no cut
+//   32 trees of 20..61, 80 k tokens of 8 x 128 bf16, 32 heads         329 MB   125 us (2.6 TB/s, 410 TFLOP/s)   14.1 us
+//   24 chains of 3..16, 138 k tokens of 8 x 128 e4m3, 64 heads        282 MB   109 us (2.6 TB/s, 313 TFLOP/s)   14.6 us
+// The wide trees' workgroups do not divide evenly over the CUs (30 % of the CU time is idle), 63 MB of partial results are written
+// and read, and 20 % of the products are padding.  Loads alone take 83 us, everything but the loads 80.
 #include "mw_kernels.h"
 
 #include <type_traits>
@@ -64,7 +73,7 @@ template <typename T> __device__ __forceinline__ u32x4 finite_only(u32x4 u, bool
 }
 template <typename T> __device__ __forceinline__ short bits_of(float x) { return __builtin_bit_cast(short, (T)x); }       // nearest even
 
-// largest of three, NaN passed over (of values that vector instructions made; written out, since the compiler first copies every
+// largest of three, a NaN passed over (of values that vector instructions made; written out, since the compiler first copies every
 // operand to quiet a NaN)
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
@@ -545,14 +554,17 @@ __device__ __forceinline__ bool find_work(const TreeAttnParams& p, int n_blocks,
     w.key1 = (int)min((long)min(u.z, p.max_pages << p.c.page_shift), (long)w.kept + last_node + 1);
     return true;
 }
-// At most 16 columns: a stream of K/V through the compute units; registers are held down for more workgroups on each.
+// At most 16 columns a workgroup: a stream of K/V through the compute units; registers are held down for more workgroups on each.
 template <typename T, bool KV8, int D>
 __global__ __launch_bounds__(256, D == 64 ? 4 : 3) void tree_attn_narrow_kernel(TreeAttnParams p, int n_blocks, int group) {
     __shared__ Shared<KV8, D> lds;
     Work w;
     if (find_work(p, n_blocks, group, 16, w)) attend<T, KV8, D, 1, 4>(p, group, w, lds);
 }
-// Up to 128 columns a workgroup; how the four waves share columns and keys goes by the columns that this request has left.
+// Up to 128 columns a workgroup; how the four waves share columns and keys goes by the columns that this request has left: a wave
+// without columns would only stage.  (A wave of 64 columns reads half as much LDS per product but spills: 250 us; eight waves
+// of 256 columns read a request's rows once: 155 us, one workgroup per CU and its barriers; eight of 16 columns each 164 us;
+// queries in LDS and two tiles in flight 156 us.)
 template <typename T, bool KV8, int D>
 __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeAttnParams p, int n_blocks, int group) {
     __shared__ Shared<KV8, D> lds;
@@ -628,6 +640,8 @@ template <typename T, bool KV8, int D>
 void launch_tree_t(const TreeAttnParams& p, hipStream_t s) {
     const int group = p.heads / p.c.heads;
     const long cols = (long)p.max_nodes * group;
+    // 24 chains over 138 k tokens, 8 K/V heads of 128, narrow / wide: 16 columns 115 / 127 us bf16, 73 / 94 us e4m3; 24 columns, two
+    // narrow blocks that read the rows twice, 166 / 131 and 106 / 96 us
     const int block = cols <= 16 ? 16 : 128;
     const int n_blocks = (int)((cols + block - 1) / block);
     const long pairs = ((long)p.n_units * p.c.heads + 7) / 8 * 8;
