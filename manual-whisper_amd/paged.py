@@ -272,7 +272,7 @@ def tree_attention(q, cache: PagedCache, table, kept, row_start, units, unit_sta
                    out=None):
     """Attention of the step's rows over one cache layer (``mw_tree_attention``): ``q`` [rows, n_heads, head_dim] -> the same
     shape.  ``row_start``, ``units``, ``unit_start`` and (trees) ``mask`` are a plan's; ``max_nodes``: the most rows a request has.
-    ``scale`` defaults to 1 / sqrt(head_dim)."""
+    ``scale`` defaults to 1 / sqrt(head_dim).  Rows behind the last request are left as they are in ``out`` (undefined without one)."""
     dev = cache._one().device
     pq, q_row, q_head = _rows3(q, "q", dev)
     rows, heads, dim = q.shape
@@ -314,7 +314,8 @@ def tree_attention(q, cache: PagedCache, table, kept, row_start, units, unit_sta
 
 def accept(logits, tokens, parents, row_start, depth: int, suppress=None):
     """Greedy acceptance of the step's trees (``mw_tree_accept``): ``logits`` [rows, vocab] (float32, float16 or bfloat16, any row
-    stride), ``tokens``, ``parents`` int32 [rows] -> best [rows], path [batch, depth], count [batch], out_tokens [batch, depth]."""
+    stride), ``tokens``, ``parents`` int32 [rows] -> best [rows] (undefined behind the last request), path [batch, depth], count
+    [batch], out_tokens [batch, depth]."""
     dev = _gpu_of(logits, "logits")
     dtype = _FLOATS.get(logits.dtype)
     if logits.dim() != 2 or dtype is None or logits.requires_grad:

@@ -73,6 +73,29 @@ def test_drafts_change_the_passes_and_not_the_ids(name, max_new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("nodes,n_prompt,max_new", [(64, 1, 40), (33, 1, 1), (64, 4, 2), (17, 2, 60)])
+def test_widest_trees_and_shortest_prompts(nodes, n_prompt, max_new):
+    """Trees over two mask words, a prompt of one token, decodes of one and two tokens; drafts right, interleaved and of several kinds."""
+    n = 2
+    dims, w, pcm, eng = _engine("micro", 2 * nodes, n)
+    orc = WhisperOracle(dims, w)
+    enc = orc.encode(log_mel(pcm, dims.n_mels))
+    base = synthetic_options(dims, max_new=max_new)
+    opts = DecodeOptions(prompt=tuple(base.prompt)[:n_prompt], suppress=base.suppress, begin_suppress=base.begin_suppress, eot=base.eot, max_new=max_new)
+    eng.set_decode_options(opts)
+    want, want_len, _ = eng.decode_greedy(n)
+    text = [want[b, :want_len[b]].tolist() for b in range(n)]
+    rng = np.random.default_rng(nodes)
+    noise = [[rng.integers(0, dims.vocab, 50).tolist() for _ in range(5)] for _ in range(n)]
+    for drafts in ([[t] for t in text], [[t, t[1:], t[2:]] + x for t, x in zip(text, noise)], noise, [[], [text[1]]]):
+        got, got_len = eng.decode_drafted(n, drafts, nodes)
+        _same_up_to_near_ties(got, want, orc, enc, opts)
+        if (got == want).all():
+            assert (got_len == want_len).all() and eng.stage_ms()["decode_steps"] <= max_new
+    eng.close()
+
+
+@pytest.mark.gpu
 def test_a_decode_without_graphs_and_one_after_other_kinds_agree():
     """The same call with and without captured passes, between greedy, beam and sampled decodes that use the same memory."""
     n = 2
