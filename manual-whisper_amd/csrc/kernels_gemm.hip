@@ -56,6 +56,14 @@ __device__ __forceinline__ int swz(int row, int chunk) {      // offset in halfs
     return row * BK + ((chunk ^ ((row >> 1) & 7)) << 3);
 }
 
+// fp32 -> fp16 of a value that has been rounded to fp32.  Left alone, the compiler joins the conversion with the product or sum
+// before it (one rounding instead of two) in some of the unrolled copies of an epilogue and not in others, and a row's values
+// would depend on its place in a tile: on what shares its pass.
+__device__ __forceinline__ f16 to_f16(float x) {
+    asm("" : "+v"(x));
+    return (f16)x;
+}
+
 // GELU(x) = x * Phi(x) with erf from Abramowitz & Stegun 7.1.26 (|error| <= 1.5e-7, far below the
 // fp16 rounding of the result); the negative side uses 1 + erf(z) = poly * exp(-z^2) directly, so
 // there is no cancellation.  12 instructions instead of the ~50 of erff: the epilogue is straight
@@ -169,7 +177,7 @@ __device__ __forceinline__ void gemm_epilogue_t(const GemmParams& p, float4v (&a
                 o.x += v[0]; o.y += v[1]; o.z += v[2]; o.w += v[3];
                 *reinterpret_cast<float4*>(c) = o;
             } else {
-                const half4 h = {(f16)v[0], (f16)v[1], (f16)v[2], (f16)v[3]};
+                const half4 h = {to_f16(v[0]), to_f16(v[1]), to_f16(v[2]), to_f16(v[3])};
                 if constexpr (OUT == OUT_F16) {
                     *reinterpret_cast<half4*>(reinterpret_cast<f16*>(p.C) + row + col[i]) = h;
                 } else if (OUT == OUT_QKV_SPLIT && sec[i] == 2) {
@@ -289,7 +297,7 @@ __device__ __forceinline__ void gemm256_epilogue_perm(const GemmParams& p, float
                 *reinterpret_cast<float4*>(c) = o0;
                 *reinterpret_cast<float4*>(c + 4) = o1;
             } else {
-                const half8 h = {(f16)v[0], (f16)v[1], (f16)v[2], (f16)v[3], (f16)v[4], (f16)v[5], (f16)v[6], (f16)v[7]};
+                const half8 h = {to_f16(v[0]), to_f16(v[1]), to_f16(v[2]), to_f16(v[3]), to_f16(v[4]), to_f16(v[5]), to_f16(v[6]), to_f16(v[7])};
                 if constexpr (OUT == OUT_F16) {
                     *reinterpret_cast<half8*>(reinterpret_cast<f16*>(p.C) + row + col[i2]) = h;
                 } else if (OUT == OUT_QKV_SPLIT && sec[i2] == 2) {       // V^T from an untransposed tile: element stores
@@ -337,7 +345,7 @@ __device__ __forceinline__ void gemm256_epilogue_vT(const GemmParams& p, float4v
             for (int g = 0; g < 2; ++g) {
                 if (!m_ok[i2][g]) continue;
                 const float4v a = acc[2 * i2 + g][j];
-                const half4 h = {(f16)(a[0] + b), (f16)(a[1] + b), (f16)(a[2] + b), (f16)(a[3] + b)};
+                const half4 h = {to_f16(a[0] + b), to_f16(a[1] + b), to_f16(a[2] + b), to_f16(a[3] + b)};
                 *reinterpret_cast<half4*>(rowp + moff[i2][g]) = h;
             }
     }
