@@ -237,8 +237,8 @@ __global__ __launch_bounds__(XV > 0 ? 512 : 1024, (XV > 0 && R == 1 && MT == 1) 
                 const float4 g = *reinterpret_cast<const float4*>(gam + c);
                 const float4 b = *reinterpret_cast<const float4*>(bet + c);
                 *reinterpret_cast<half4*>(xs + r * ldx + c) =
-                    half4{(f16)(v[t][j].x * rstd * g.x + b.x), (f16)(v[t][j].y * rstd * g.y + b.y),
-                          (f16)(v[t][j].z * rstd * g.z + b.z), (f16)(v[t][j].w * rstd * g.w + b.w)};
+                    half4{to_f16(v[t][j].x * rstd * g.x + b.x), to_f16(v[t][j].y * rstd * g.y + b.y),
+                          to_f16(v[t][j].z * rstd * g.z + b.z), to_f16(v[t][j].w * rstd * g.w + b.w)};
             }
         }
         __syncthreads();
@@ -303,7 +303,7 @@ __global__ __launch_bounds__(XV > 0 ? 512 : 1024, (XV > 0 && R == 1 && MT == 1) 
             *reinterpret_cast<float4*>(p.out32 + (long)m * p.N + n) =
                 make_float4(res4[t].x + v[0], res4[t].y + v[1], res4[t].z + v[2], res4[t].w + v[3]);
         } else {
-            const half4 h = {(f16)v[0], (f16)v[1], (f16)v[2], (f16)v[3]};
+            const half4 h = {to_f16(v[0]), to_f16(v[1]), to_f16(v[2]), to_f16(v[3])};
             if (p.out_mode == GV_F16) {
                 *reinterpret_cast<half4*>(p.out16 + (long)m * p.N + n) = h;
             } else {   // GV_QKV: q -> out16 [B][D]; k, v -> this layer's cache at the current position
@@ -635,7 +635,7 @@ __global__ __launch_bounds__(kDecGemmWaves * 64) void gemm_dec_kernel(GemvParams
             const float4 r4 = res4[t];
             *reinterpret_cast<float4*>(p.out32 + (long)m * p.N + n) = make_float4(r4.x + o[0], r4.y + o[1], r4.z + o[2], r4.w + o[3]);
         } else {
-            const half4 h = {(f16)o[0], (f16)o[1], (f16)o[2], (f16)o[3]};
+            const half4 h = {to_f16(o[0]), to_f16(o[1]), to_f16(o[2]), to_f16(o[3])};
             if (p.out_mode == GV_F16) {
                 *reinterpret_cast<half4*>(p.out16 + (long)m * p.N + n) = h;
             } else {   // GV_QKV: q -> out16 [B][D]; k, v -> this layer's cache at the current position

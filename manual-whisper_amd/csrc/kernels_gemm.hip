@@ -56,14 +56,6 @@ __device__ __forceinline__ int swz(int row, int chunk) {      // offset in halfs
     return row * BK + ((chunk ^ ((row >> 1) & 7)) << 3);
 }
 
-// fp32 -> fp16 of a value that has been rounded to fp32.  Left alone, the compiler joins the conversion with the product or sum
-// before it (one rounding instead of two) in some of the unrolled copies of an epilogue and not in others, and a row's values
-// would depend on its place in a tile: on what shares its pass.
-__device__ __forceinline__ f16 to_f16(float x) {
-    asm("" : "+v"(x));
-    return (f16)x;
-}
-
 // GELU(x) = x * Phi(x) with erf from Abramowitz & Stegun 7.1.26 (|error| <= 1.5e-7, far below the
 // fp16 rounding of the result); the negative side uses 1 + erf(z) = poly * exp(-z^2) directly, so
 // there is no cancellation.  12 instructions instead of the ~50 of erff: the epilogue is straight

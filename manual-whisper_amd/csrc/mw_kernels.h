@@ -29,6 +29,14 @@ __device__ __forceinline__ unsigned pack4_e4m3(float a, float b, float c, float 
     return (unsigned)w;
 }
 
+// fp32 -> fp16 of a value that has been rounded to fp32.  Left alone, the compiler joins the conversion with the product or sum
+// before it (one rounding instead of two) in some copies of an unrolled epilogue and not in others, and a row's values would
+// depend on its place in a tile: on what shares its pass.
+__device__ __forceinline__ f16 to_f16(float x) {
+    asm("" : "+v"(x));
+    return (f16)x;
+}
+
 // ---------------------------------------------------------------- log-mel
 struct MelTables {
     const float* basis_cos;   // [400][256]  hann[n]*cos(2*pi*f*n/400), zero for f >= 201
