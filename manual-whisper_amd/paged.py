@@ -283,7 +283,7 @@ def tree_attention(q, cache: PagedCache, table, kept, row_start, units, unit_sta
     pt, batch, columns, t_stride = _table(table, dev)
     n_units = units.shape[0]
     if out is None:
-        out = torch.empty((rows, heads, dim), dtype=q.dtype, device=q.device)
+        out = q.new_empty(rows, heads, dim)
         po, o_row, o_head = out.data_ptr(), heads * dim, dim
     else:
         if out.shape != q.shape or out.dtype is not q.dtype:
