@@ -213,8 +213,8 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
                 hi = widen8<T>(rv[i][2], rv[i][3]);
             }
             if (kv0 + KT > min(kept, key1) || !ok) {                    // (uniform) tiles with rows of this step, or behind the last key
-                // V's infinities and NaN are held back here: in the product they would reach rows that do not see them (0 times
-                // NaN is NaN).  The rows that do get them at the end.  What lies behind the last key may be anything.
+                // V's infinities and NaN are held back here, kept tokens' too: in the product they would reach rows that do not see them
+                // (0 times NaN is NaN).  The rows that do get them at the end.  What lies behind the last key may be anything.
                 const u32x4 none = {0, 0, 0, 0};
                 if (kv0 + row >= key1 || !ok) lo = hi = none;
                 lo = finite_only<T>(lo, bad);
@@ -489,7 +489,8 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
     }
     if constexpr (WK == 1) __syncthreads();
     if (lds.bad_v) {                                         // (written before the last barrier)
-        for (int key = max(key0, kept); key < key1; ++key) {
+        // from the first tile that store_tile held something back in: kept tokens share it with the step's rows
+        for (int key = max(key0, min(kept, key1) & ~(KT - 1)); key < key1; ++key) {
             const int pgid = pages[key >> p.c.page_shift];
             if (pgid < 0 || pgid >= p.c.n_pages) continue;
             const long at = (long)pgid * p.c.page_stride + w.g * p.c.head_stride + (long)(key & page_mask) * p.c.token_stride;

@@ -804,3 +804,50 @@ def test_calls_on_other_streams_and_in_graphs():
         assert all(torch.equal(a, b) for a, b in zip(now, eager[turn]))
         for k in range(2):
             assert all(torch.equal(a, b) for a, b in zip(outs[k], eager[(turn + k) % 3])), (turn, k)
+
+
+KEPT_POISON = [  # kept, nodes, heads, kv heads, page, target of the cut, table columns (None: all), poisoned kept positions of request 0
+    (70, 4, 4, 2, 16, 0, None, (3, 64, 66, 69)),              # a tile that kept tokens share with the nodes, and the tile before it
+    (70, 1, 4, 2, 64, 0, None, (65,)),
+    (63, 9, 4, 2, 32, 0, None, (0, 62)),
+    (200, 20, 8, 2, 16, 0, None, (192, 199)),
+    (130, 40, 4, 2, 16, 0, None, (5, 128, 129)),
+    (700, 7, 4, 2, 16, 6, None, (130, 640, 699)),             # cut into pieces
+    (90, 3, 4, 2, 16, 0, 5, (64, 70, 79)),                    # the table ends before the kept tokens do
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,cache_kind", [("f16", "f16"), ("bf16", "bf16"), ("f16", "e4m3")])
+@pytest.mark.parametrize("tree", [True, False], ids=["tree", "chain"])
+@pytest.mark.parametrize("case", range(len(KEPT_POISON)))
+def test_infinities_and_nan_of_kept_tokens_reach_every_row(case, tree, kind, cache_kind):
+    """All rows see every kept token: a value of V there that is no finite number leaves none of the request's results at its head and
+    dimension finite, wherever the token lies in a tile; every other result keeps its bits."""
+    from manual_whisper_amd import paged
+    kept0, nodes, heads, kv, page, target, columns, places = KEPT_POISON[case]
+    rng = np.random.default_rng(case)
+    kept, n, dim = [kept0, 17], [nodes, min(nodes, 3)], 64
+    table, n_pages, start, see, words = _tree_case(rng, kept, n, page)
+    cache, _, _ = _new_cache(rng, cache_kind, (n_pages, kv, page, dim))
+    q = torch.randn(start[-1], heads, dim, device="cuda").to(DT[kind])
+    units, first = _units(kept, n, target, 64)
+    dev_table = _dev([r[:columns] for r in table] if columns else table)
+
+    def attend():
+        return paged.tree_attention(q, cache, dev_table, _dev(kept), _dev(start), units, first, nodes, mask=_pack(see) if tree else None)
+
+    clean = attend()
+    for i, place in enumerate(places):
+        pg, o = table[0][place // page], place % page
+        bads = [0x7F, 0xFF] if cache_kind == "e4m3" else [float("inf"), float("nan"), float("-inf")]
+        for bad in bads:
+            d, g = (7 * i + 3) % dim, i % kv
+            before = cache.v[pg, g, o, d].clone()
+            cache.v[pg, g, o, d] = bad
+            got = attend()
+            cache.v[pg, g, o, d] = before
+            hit = torch.zeros_like(got, dtype=torch.bool)
+            hit[:start[1], g * (heads // kv):(g + 1) * (heads // kv), d] = True
+            assert not torch.isfinite(got[hit]).any(), (place, bad)
+            assert torch.equal(got[~hit], clean[~hit]), (place, bad)
