@@ -242,9 +242,11 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
     float ref[QT], gap[QT], l[QT];
 #pragma unroll
     for (int qs = 0; qs < QT; ++qs) { ref[qs] = 0.f; gap[qs] = -INFINITY; l[qs] = 0.f; }
-    // e4m3: weights are p_j times V's row scale relative to a power of two above every scale seen so far, so that they stay
-    // within fp16's range whatever the scales are; the accumulators are multiplied by it at the end
-    float vref = 0.f;
+    // e4m3: weights are p_j times V's row scale relative to a power of two above every scale that the column has seen so far, so
+    // that they stay within fp16's range whatever the scales are; the accumulators are multiplied by it at the end
+    float vref[QT];
+#pragma unroll
+    for (int qs = 0; qs < QT; ++qs) vref[qs] = 0.f;
     // which of the 64 keys from node `first` on (negative: kept tokens before it) the row of node `n` sees
     auto visible = [&](int n, int first) -> unsigned long long {
         if (first <= -64) return ~0ull;
@@ -339,28 +341,48 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
             for (int i = 0; i < NK; ++i) top[qs] = max3(max3(top[qs], sc[i][qs][0], sc[i][qs][1]), sc[i][qs][2], sc[i][qs][3]);
             lift = lift || top[qs] > gap[qs];
         }
-        float big = 0.f;                                     // e4m3: V's largest row scale in this tile, the same in all lanes
+        float big[QT];                                       // e4m3: V's largest row scale in this tile among the keys that a column sees
         if constexpr (KV8) {
+            if (kv0 + KT > kept) {
 #pragma unroll
-            for (int i = 0; i < NK; ++i) {
-                const float4v s4 = *reinterpret_cast<const float4v*>(&lds.scales[1][(wk * NK + i) * 16 + 4 * fg]);
-                big = fmaxf(big, fmaxf(fmaxf(s4[0], s4[1]), fmaxf(s4[2], s4[3])));
+                for (int qs = 0; qs < QT; ++qs) {
+                    big[qs] = 0.f;
+#pragma unroll
+                    for (int i = 0; i < NK; ++i) {
+                        const float4v s4 = *reinterpret_cast<const float4v*>(&lds.scales[1][(wk * NK + i) * 16 + 4 * fg]);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) big[qs] = fmaxf(big[qs], sc[i][qs][r] == -INFINITY ? 0.f : s4[r]);
+                    }
+                    big[qs] = column_max(big[qs]);
+                }
+            } else {                                         // kept tokens: every column sees all of them (0 where there is none)
+                float all = 0.f;
+#pragma unroll
+                for (int i = 0; i < NK; ++i) {
+                    const float4v s4 = *reinterpret_cast<const float4v*>(&lds.scales[1][(wk * NK + i) * 16 + 4 * fg]);
+                    all = fmaxf(all, fmaxf(fmaxf(s4[0], s4[1]), fmaxf(s4[2], s4[3])));
+                }
+                all = column_max(all);
+#pragma unroll
+                for (int qs = 0; qs < QT; ++qs) big[qs] = all;
             }
-            big = column_max(big);
+#pragma unroll
+            for (int qs = 0; qs < QT; ++qs) lift = lift || big[qs] > vref[qs];
         }
-        if (__any(lift) || big > vref) {                     // wave-uniform
-            float f = 1.f;
-            if (KV8 && big > vref) {
-                const float up = __uint_as_float(min((__float_as_uint(big) & 0x7f800000u) + 0x00800000u, 0x7f000000u));
-                f = vref / up;
-                vref = up;
-            }
+        if (__any(lift)) {                                   // wave-uniform; a column moves for what it sees itself only
 #pragma unroll
             for (int qs = 0; qs < QT; ++qs) {
+                float f = 1.f;
+                if (KV8 && big[qs] > vref[qs]) {
+                    const float up = __uint_as_float(min((__float_as_uint(big[qs]) & 0x7f800000u) + 0x00800000u, 0x7f000000u));
+                    f = vref[qs] / up;
+                    vref[qs] = up;
+                }
                 const float up = column_max(top[qs]);
-                const float to = ref[qs] + (gap[qs] > 0.f ? fmaxf(up, 0.f) : up == -INFINITY ? 0.f : up), d = to - ref[qs];
+                const bool rises = up > gap[qs];
+                const float to = ref[qs] + (rises ? up : 0.f), d = to - ref[qs];
                 const float alpha = gap[qs] > 0.f ? __builtin_amdgcn_exp2f(-d) : 1.f;
-                if (up > -INFINITY) gap[qs] = kGap;
+                if (rises) gap[qs] = kGap;
                 ref[qs] = to;
 #pragma unroll
                 for (int i = 0; i < NK; ++i)
@@ -371,15 +393,19 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
                 for (int d = 0; d < ND; ++d) { o[d][qs][0] *= alpha * f; o[d][qs][1] *= alpha * f; o[d][qs][2] *= alpha * f; o[d][qs][3] *= alpha * f; }
             }
         }
-        const float vinv = KV8 && vref > 0.f ? 1.f / vref : 0.f;              // (a power of two)
+        float vinv[QT];                                      // (powers of two)
+#pragma unroll
+        for (int qs = 0; qs < QT; ++qs) vinv[qs] = KV8 && vref[qs] > 0.f ? 1.f / vref[qs] : 0.f;
         auto weigh = [&](auto some_unseen) {
+            constexpr bool EDGE = decltype(some_unseen)::value;
 #pragma unroll
             for (int i = 0; i < NK; ++i) {
                 float4v vs4 = float4v{1, 1, 1, 1};
                 if constexpr (KV8) {
                     vs4 = *reinterpret_cast<const float4v*>(&lds.scales[1][(wk * NK + i) * 16 + 4 * fg]);
+                    if constexpr (!EDGE)                     // kept tokens only so far: the columns' references are the same
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) vs4[r] *= vinv;
+                        for (int r = 0; r < 4; ++r) vs4[r] *= vinv[0];
                 }
 #pragma unroll
                 for (int qs = 0; qs < QT; ++qs)
@@ -388,7 +414,8 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
                         const float e = __builtin_amdgcn_exp2f(sc[i][qs][r]);
                         l[qs] += e;                          // of this lane's keys; the column's sum is formed at the end
                         if constexpr (!KV8) sc[i][qs][r] = e;
-                        else sc[i][qs][r] = decltype(some_unseen)::value && e == 0.f ? 0.f : e * vs4[r];       // whatever the scale of an unseen key
+                        else if constexpr (!EDGE) sc[i][qs][r] = e * vs4[r];
+                        else sc[i][qs][r] = e == 0.f ? 0.f : e * (vs4[r] * vinv[qs]);          // whatever the scale of an unseen key
                     }
             }
         };
@@ -447,7 +474,7 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
         l[qs] = column_sum(l[qs]);
         if constexpr (KV8)
 #pragma unroll
-            for (int d = 0; d < ND; ++d) { o[d][qs][0] *= vref; o[d][qs][1] *= vref; o[d][qs][2] *= vref; o[d][qs][3] *= vref; }
+            for (int d = 0; d < ND; ++d) { o[d][qs][0] *= vref[qs]; o[d][qs][1] *= vref[qs]; o[d][qs][2] *= vref[qs]; o[d][qs][3] *= vref[qs]; }
     }
     constexpr int DW = ND / WK;                              // 16-dim tiles of the result that a wave ends up with
     const int d0 = WK > 1 ? wk * DW : 0;

@@ -851,3 +851,41 @@ def test_infinities_and_nan_of_kept_tokens_reach_every_row(case, tree, kind, cac
             hit[:start[1], g * (heads // kv):(g + 1) * (heads // kv), d] = True
             assert not torch.isfinite(got[hit]).any(), (place, bad)
             assert torch.equal(got[~hit], clean[~hit]), (place, bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("nodes,heads", [(6, 2), (20, 4), (40, 8)])
+@pytest.mark.parametrize("target", [0, 4])
+def test_row_scales_of_nodes_that_a_row_does_not_see_stay_away(nodes, heads, target, kind):
+    """e4m3: a node of one branch whose V has a row scale far above the others' (or an infinite one) leaves the bits of the rows that
+    do not see it; those that see a finite one are right."""
+    from manual_whisper_amd import paged
+    rng = np.random.default_rng(nodes)
+    kept, n, page, kv, dim = [21, 164], [nodes, nodes], 16, 2, 64
+    table, n_pages, start, _, words = _tree_case(rng, kept, n, page)
+    see = np.zeros((start[-1], words * 32), bool)
+    for b in range(2):                                        # two branches under the root: odd nodes and even nodes
+        for i in range(nodes):
+            see[start[b] + i, 0] = True
+            see[start[b] + i, 2 - i % 2:i + 1:2] = True
+            see[start[b] + i, i] = True
+    cache, _, _ = _new_cache(rng, "e4m3", (n_pages, kv, page, dim))
+    q = torch.randn(start[-1], heads, dim, device="cuda").to(DT[kind])
+    units, first = _units(kept, n, target, 64)
+    args = (_dev(table), _dev(kept), _dev(start), units, first, nodes)
+    clean = paged.tree_attention(q, cache, *args, mask=_pack(see))
+    sees = torch.tensor(see[:, 3], device="cuda")
+    ordinary = float(cache.v_scale.max())
+    for factor in (2.0 ** 7, 2.0 ** 14, 2.0 ** 25, 2.0 ** 100, float("inf")):
+        for b in range(2):
+            at = kept[b] + 3
+            cache.v_scale[table[b][at // page], :, at % page] = ordinary * factor
+        got = paged.tree_attention(q, cache, *args, mask=_pack(see))
+        assert torch.equal(got[~sees], clean[~sees]), factor
+        if factor <= 2.0 ** 14 and kind == "bf16":            # (fp16 results may be infinite)
+            want, size, big, _ = ref.attention(q.double().cpu().numpy(), _values(cache, "k"), _values(cache, "v"), table, page, kept, start, see)
+            # weights and results rounded once each (u); scores and sums as in _close
+            u, keys = torch.finfo(DT[kind]).eps / 2, max(kept) + nodes
+            tol = (2.01 * u + 2 * (dim + 8) * 2.0 ** -24 * (1 + big) + 2 * (keys + 64) * 2.0 ** -24) * size + u * np.abs(want) * 1e-2
+            assert (np.abs(got.double().cpu().numpy() - want) <= tol).all(), factor
