@@ -39,8 +39,12 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int KT = 64;                                       // keys of a tile
-constexpr float kGap = 6.f;                                  // positive: gap > 0 says that a column has seen a key
 
+// Weights are 2^(score - reference).  When a column's reference moves it goes kLow below the largest score, and it stays until a
+// score is more than kGap above it (positive: gap > 0 says that a column has seen a key).  fp16 holds full precision from 2^-14 to
+// 2^15, so its weights are kept high: the largest is 2^10 .. 2^14 (twice that beside an e4m3 row scale above 2^127), and one is
+// rounded by more than half a step of the type only where it is below 2^-24 of the largest, then by at most 2^-35 of it.  (With the
+// largest near 1 a long cache beside one dominant key loses its weights: 20 k tokens of e^-18 each came out as nothing.)
 template <typename T> struct Mat;
 template <> struct Mat<f16> {
     static __device__ __forceinline__ float4v mma32(short8v a, short8v b, float4v c) {
@@ -50,6 +54,7 @@ template <> struct Mat<f16> {
         return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(half4, a), __builtin_bit_cast(half4, b), c, 0, 0, 0);
     }
     static constexpr unsigned kExp = 0x7c007c00u;            // exponents of a pair of values
+    static constexpr float kLow = 10.f, kGap = 14.f;
 };
 template <> struct Mat<bf16> {
     static __device__ __forceinline__ float4v mma32(short8v a, short8v b, float4v c) {
@@ -59,6 +64,7 @@ template <> struct Mat<bf16> {
         return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
     }
     static constexpr unsigned kExp = 0x7f807f80u;
+    static constexpr float kLow = 0.f, kGap = 6.f;           // (the range of fp32)
 };
 // eight values with 0 in the place of infinities and NaN (all bits of the exponent set); `any`: whether there were some
 template <typename T> __device__ __forceinline__ u32x4 finite_only(u32x4 u, bool& any) {
@@ -380,9 +386,9 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
                 }
                 const float up = column_max(top[qs]);
                 const bool rises = up > gap[qs];
-                const float to = ref[qs] + (rises ? up : 0.f), d = to - ref[qs];
+                const float to = ref[qs] + (rises ? up - Mat<T>::kLow : 0.f), d = to - ref[qs];
                 const float alpha = gap[qs] > 0.f ? __builtin_amdgcn_exp2f(-d) : 1.f;
-                if (rises) gap[qs] = kGap;
+                if (rises) gap[qs] = Mat<T>::kGap;
                 ref[qs] = to;
 #pragma unroll
                 for (int i = 0; i < NK; ++i)
@@ -422,8 +428,8 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
         if (KV8 && edge) weigh(std::true_type{});
         else weigh(std::false_type{});
         __builtin_amdgcn_sched_barrier(0);
-        // ---- O^T += V^T P^T.  The weights are rounded once to T (half a step of T each, as the result is); the sum above is of
-        // the unrounded ones.
+        // ---- O^T += V^T P^T.  The weights are rounded once to T (half a step of T, for fp16 down to 2^-24 of the largest); the sum
+        // above is of the unrounded ones.
         const short* const vt = ldsV;
         {
             typedef short4v __attribute__((address_space(3)))* lds4;

@@ -889,3 +889,45 @@ def test_row_scales_of_nodes_that_a_row_does_not_see_stay_away(nodes, heads, tar
             u, keys = torch.finfo(DT[kind]).eps / 2, max(kept) + nodes
             tol = (2.01 * u + 2 * (dim + 8) * 2.0 ** -24 * (1 + big) + 2 * (keys + 64) * 2.0 ** -24) * size + u * np.abs(want) * 1e-2
             assert (np.abs(got.double().cpu().numpy() - want) <= tol).all(), factor
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,cache_kind", [("f16", "f16"), ("bf16", "bf16"), ("f16", "e4m3")])
+@pytest.mark.parametrize("nats", [12, 16, 18])
+@pytest.mark.parametrize("nodes,heads", [(2, 2), (20, 2), (45, 2)])
+def test_small_weights_beside_a_dominant_key(nodes, heads, nats, kind, cache_kind):
+    """A long cache whose first token draws nearly all of the attention and has a V of zeros, every other token the same small weight:
+    the result is what the small weights add up to."""
+    from manual_whisper_amd import paged
+    rng = np.random.default_rng(nats)
+    kept, page, dim = 20000, 64, 64
+    n_pages = -(-(kept + nodes) // page)
+    k = np.zeros((n_pages, 1, page, dim), np.float32)
+    v = rng.uniform(0.5, 1.5, k.shape).astype(np.float32)
+    k[0, 0, 0] = 1.0
+    v[0, 0, 0] = 0
+    q = torch.full((nodes, heads, dim), 0.25, dtype=DT[kind], device="cuda")
+    scale = nats / (dim * 0.25)                               # scores: `nats` of the first token, zero of the others
+    if cache_kind == "e4m3":
+        one = torch.ones(k.shape[:-1], dtype=torch.float32, device="cuda")
+        cache = paged.PagedCache(*(torch.tensor(x, device="cuda").to(torch.float8_e4m3fn).view(torch.uint8) for x in (k, v)), one, one.clone())
+    else:
+        cache = paged.PagedCache(*(torch.tensor(x, device="cuda").to(DT[kind]) for x in (k, v)))
+    table, start = [rng.permutation(n_pages).tolist()], [0, nodes]
+    table[0].remove(0)
+    table[0].insert(0, 0)                                     # page 0 holds the first token
+    units, first = _units([kept], [nodes], 0, 64)
+    got = paged.tree_attention(q, cache, _dev(table), _dev([kept]), _dev(start), units, first, nodes, scale=scale).double().cpu().numpy()
+    kk, vv = _values(cache, "k")[table[0], 0].reshape(-1, dim), _values(cache, "v")[table[0], 0].reshape(-1, dim)
+    s = kk @ np.full(dim, 0.25) * scale
+    u, tiles = torch.finfo(DT[kind]).eps / 2, -(-(kept + nodes) // 64)
+    for i in range(nodes):
+        p = np.exp(s[:kept + i + 1] - s.max())
+        want = p @ vv[:kept + i + 1] / p.sum()
+        # the weights are rounded once, the result once (u each); the score of the first token, 18 log2 e = 26, carries 2 roundings of
+        # 2^-24 and so does the exponent; up to 65 roundings a tile on the way of a value into its sum; fp16 weights below 2^-14 are off
+        # by 2^-25 where the largest is 2^10 at least (e4m3: times V's scale relative to a power of two, at most 2 above it)
+        tol = (2.01 * u + 4 * 26 * 2.0 ** -24 + 2 * 65 * tiles * 2.0 ** -24) * want
+        if kind == "f16":
+            tol = tol + (kept + nodes) * 2.0 ** -35 * (2 if cache_kind == "e4m3" else 1) * 1.5 + 2.0 ** -25
+        assert (np.abs(got[i] - want) <= tol).all(), (i, float((np.abs(got[i] - want) / tol).max()))
