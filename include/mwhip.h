@@ -389,7 +389,9 @@ typedef struct {
     int32_t max_nodes;                    /* no request has more rows (more are not computed)                           */
     const int32_t* table; int64_t table_stride; int32_t max_pages;          /* max_pages * page_size < 2^31 - 4096       */
     const int32_t* kept; const int32_t* row_start;
-    const int32_t* units; const int32_t* unit_start; int32_t n_units;       /* of mw_paged_plan; n_units = batch + chunk_units */
+    const int32_t* units; const int32_t* unit_start; int32_t n_units;       /* of mw_paged_plan; n_units = batch + chunk_units, or
+                                           * fewer, but unit_start[batch] at least; with no more than batch (no workspace) the
+                                           * first unit of a request that was cut takes all of its keys                 */
     const uint32_t* mask; int32_t mask_words;                   /* NULL: chains (node i sees nodes 0..i)                 */
     float scale;                          /* of the scores, usually 1 / sqrt(head_dim)                                  */
     void* workspace; int64_t workspace_bytes;       /* mw_tree_attention_workspace() bytes, 16-byte aligned              */

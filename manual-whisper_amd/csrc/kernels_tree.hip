@@ -547,7 +547,7 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
     for (int qs = 0; qs < QT; ++qs) {
         const int c = w.col0 + (wq * QT + qs) * 16 + fr;
         if (c >= w.cols) continue;
-        if (w.pieces <= 1 || !p.workspace) {
+        if (w.pieces <= 1) {
             const float inv = l[qs] == 0.f ? 0.f : 1.f / l[qs];               // (a NaN sum stays NaN)
             short* dst = static_cast<short*>(p.out) + (long)(w.row0 + node[qs]) * p.out_row + (long)(w.g * group + c - node[qs] * group) * p.out_head;
 #pragma unroll
@@ -573,7 +573,11 @@ __device__ __forceinline__ bool find_work(const TreeAttnParams& p, int n_blocks,
     const int pair = blockIdx.x / (8 * n_blocks) * 8 + (blockIdx.x & 7), cb = (blockIdx.x >> 3) % n_blocks;
     w.unit = pair / p.c.heads; w.g = pair - w.unit * p.c.heads;
     if (w.unit >= p.n_units) return false;
-    const int4 u = reinterpret_cast<const int4*>(p.units)[w.unit];
+    int4 u = reinterpret_cast<const int4*>(p.units)[w.unit];
+    if (u.w > 1 && !p.workspace) {                           // no room for partial results: the first unit takes the whole request
+        if (u.y > 0) return false;
+        u.z = 0x7fffffff; u.w = 1;
+    }
     w.b = u.x; w.pieces = u.w;
     if (w.b < 0 || w.b >= p.batch) return false;
     w.row0 = max(0, p.row_start[w.b]);

@@ -350,7 +350,7 @@ struct TreeAttnParams {
     int n_units;
     const unsigned* mask; int mask_words;                      // null: chains
     float scale;
-    float* workspace;                                          // tree_attn_workspace() bytes; not read when no request is cut
+    float* workspace;                                          // tree_attn_workspace() bytes; null where that is 0
 };
 // Drafted greedy decoding: one context's state.  Trees have `nodes` rows each, so row r belongs to recording r / nodes.
 constexpr int kMaxDrafts = 8, kMaxTreeNodes = 64;              // powers of two; a tree fits one wave

@@ -162,7 +162,7 @@ extern "C" int mw_tree_attention(const mw_tree_args* a, int device, void* stream
     p.max_nodes = a->max_nodes; p.q = a->q; p.q_row = a->q_row_stride; p.q_head = a->q_head_stride; p.out = a->out;
     p.out_row = a->out_row_stride; p.out_head = a->out_head_stride; p.table = a->table; p.table_stride = a->table_stride; p.max_pages = a->max_pages;
     p.kept = a->kept; p.row_start = a->row_start; p.units = a->units; p.unit_start = a->unit_start; p.n_units = a->n_units;
-    p.mask = a->mask; p.mask_words = a->mask ? a->mask_words : 0; p.scale = a->scale; p.workspace = static_cast<float*>(a->workspace);
+    p.mask = a->mask; p.mask_words = a->mask ? a->mask_words : 0; p.scale = a->scale; p.workspace = need ? static_cast<float*>(a->workspace) : nullptr;
     launch_tree_attention(p, static_cast<hipStream_t>(stream));
     return launched(who, hipGetLastError());
 }

@@ -931,3 +931,33 @@ def test_small_weights_beside_a_dominant_key(nodes, heads, nats, kind, cache_kin
         if kind == "f16":
             tol = tol + (kept + nodes) * 2.0 ** -35 * (2 if cache_kind == "e4m3" else 1) * 1.5 + 2.0 ** -25
         assert (np.abs(got[i] - want) <= tol).all(), (i, float((np.abs(got[i] - want) / tol).max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fresh", [3, 20])
+def test_cut_requests_among_idle_ones_without_a_workspace(fresh):
+    """No more units than requests, and still one request in several pieces (the others are idle): it is attended to as a whole, and a
+    workspace that the call does not ask for is not written."""
+    from manual_whisper_amd import paged
+    rng = np.random.default_rng(fresh)
+    kept, n, page, heads, kv, dim = [10, 700, 0, 90], [0, fresh, 0, 0], 16, 4, 2, 64
+    table, n_pages, start, see, words = _tree_case(rng, kept, n, page)
+    cache, k, v = _new_cache(rng, "f16", (n_pages, kv, page, dim))
+    q = torch.randn(fresh, heads, dim, device="cuda", dtype=torch.float16)
+    want, size, big, vmax = ref.attention(q.double().cpu().numpy(), k, v, table, page, kept, start, see)
+    dev = [_dev(table), _dev(kept), _dev(start)]
+    mask, c = _pack(see), cache
+    for pieces in (2, 3, 4):
+        units, first = _units(kept, n, pieces, 64)
+        assert first.tolist() == [0, 0, pieces, pieces, pieces]
+        units = units[:pieces].contiguous()
+        got = paged.tree_attention(q, cache, *dev, units, first, fresh, mask=mask)
+        _close(got.double().cpu().numpy(), want, size, big, vmax, "f16", dim, 700 + fresh, False)
+        guard, out = torch.full((1 << 20,), 7.0, device="cuda"), torch.zeros_like(q)
+        one = _lib.PagedCache(c.k.data_ptr(), c.v.data_ptr(), None, None, *c.k.stride()[:3], n_pages, page, kv, dim, 1)
+        a = _lib.TreeArgs(one, q.data_ptr(), heads * dim, dim, out.data_ptr(), heads * dim, dim, 1, heads, fresh, 4, fresh, dev[0].data_ptr(),
+                          dev[0].shape[1], dev[0].shape[1], dev[1].data_ptr(), dev[2].data_ptr(), units.data_ptr(), first.data_ptr(), pieces,
+                          mask.data_ptr(), words, dim ** -0.5, guard.data_ptr(), 16)
+        assert _lib.load().mw_tree_attention_workspace(C.byref(a)) == 0
+        assert _lib.load().mw_tree_attention(C.byref(a), 0, torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(out, got) and (guard == 7).all()
