@@ -1001,14 +1001,14 @@ struct DraftPass { int rows, max_nodes, table_cols; const unsigned* mask; int ma
 static void draft_self_attention(mw_ctx* ctx, int li, const f16* qkv, f16* out, const DraftPass& dp) {
     const int D = ctx->d.d_model;
     const PagedCacheView c = draft_cache(ctx, li);
-    launch_paged_write(c, kHeadDim, 0, qkv + D, qkv + 2 * D, 3L * D, kHeadDim, 3L * D, kHeadDim, ctx->dr_slots, dp.rows, ctx->stream);
+    (void)launch_paged_write(c, kHeadDim, 0, qkv + D, qkv + 2 * D, 3L * D, kHeadDim, 3L * D, kHeadDim, ctx->dr_slots, dp.rows, ctx->stream);
     TreeAttnParams p{};
     p.c = c; p.dim = kHeadDim; p.heads = ctx->d.n_heads; p.rows = dp.rows; p.batch = ctx->dr.n_audio; p.max_nodes = dp.max_nodes;
     p.q = qkv; p.q_row = 3L * D; p.q_head = kHeadDim; p.out = out; p.out_row = D; p.out_head = kHeadDim;
     p.table = ctx->dr_table; p.table_stride = dp.table_cols; p.max_pages = dp.table_cols; p.kept = ctx->dr.kept; p.row_start = ctx->dr_row_start;
     p.units = ctx->dr_units; p.unit_start = ctx->dr_unit_start; p.n_units = ctx->dr.n_audio;       // short caches: no request is cut
     p.mask = dp.mask; p.mask_words = dp.mask_words; p.scale = 1.f;
-    launch_tree_attention(p, ctx->stream);
+    (void)launch_tree_attention(p, ctx->stream);
 }
 
 static void enqueue_layer(mw_ctx* ctx, int li, int B, bool want_logits, const FinalizeParams& fp, int max_keys, const BeamParams* beam,
@@ -1416,7 +1416,7 @@ static void enqueue_draft_tail(mw_ctx* ctx, int rows, const int* row_start, int 
     a.suppress = suppress; a.tokens = ctx->dr.tokens; a.parents = ctx->dr.parents; a.row_start = row_start;
     a.best = ctx->dr_best; a.path = ctx->dr_path; a.count = const_cast<int*>(ctx->dr.count); a.out_tokens = const_cast<int*>(ctx->dr.out_tokens);
     a.workspace = ctx->dr_work;
-    launch_tree_accept(a, s);
+    (void)launch_tree_accept(a, s);
 }
 static void enqueue_draft_step(mw_ctx* ctx, int table_cols) {
     const mw_model_desc& d = ctx->d;
@@ -1424,13 +1424,13 @@ static void enqueue_draft_step(mw_ctx* ctx, int table_cols) {
     const int rows = r.n_audio * r.nodes;
     hipStream_t s = ctx->stream;
     const DraftPass pass{rows, r.nodes, table_cols, ctx->dr_mask, (r.nodes + 31) / 32};
-    launch_paged_plan(draft_plan(ctx, rows, table_cols, true), s);
+    (void)launch_paged_plan(draft_plan(ctx, rows, table_cols, true), s);
     launch_draft_embed(r.tokens, ctx->dr_positions, ctx->tok_emb, ctx->dec_pos, d.d_model, d.n_text_ctx, ctx->dx, rows, s);
     const FinalizeParams fp{};
     for (int li = 0; li < d.dec_layers; ++li) enqueue_layer(ctx, li, rows, false, fp, 0, nullptr, kLayerGemv | kLayerAttn, nullptr, &pass);
     enqueue_draft_tail(ctx, rows, ctx->dr_row_start, r.nodes, ctx->mask_rest);
-    launch_paged_compact(draft_cache(ctx, 0), d.dec_layers, (long)ctx->max_batch * d.d_model * d.n_text_ctx, 0, kHeadDim, ctx->dr_table, table_cols,
-                         table_cols, r.kept, ctx->dr_path, r.nodes, r.count, r.n_audio, s);
+    (void)launch_paged_compact(draft_cache(ctx, 0), d.dec_layers, (long)ctx->max_batch * d.d_model * d.n_text_ctx, 0, kHeadDim, ctx->dr_table, table_cols,
+                               table_cols, r.kept, ctx->dr_path, r.nodes, r.count, r.n_audio, s);
     launch_draft_step(r, r.nodes, 0, s);
 }
 
@@ -1494,7 +1494,7 @@ extern "C" int mw_decode_drafted(mw_ctx* ctx, int n_audio, int nodes, const int3
     HIPCHK(hipStreamSynchronize(s));
     HIPCHK(hipEventRecord(ctx->ev[3], s));
     launch_draft_init(r, P, s);
-    launch_paged_plan(draft_plan(ctx, n_audio * P, table_cols, false), s);
+    (void)launch_paged_plan(draft_plan(ctx, n_audio * P, table_cols, false), s);
     const DraftPass prompt{n_audio * P, P, table_cols, nullptr, 0};
     int rc = run_prefill(ctx, n_audio, P, 1, nullptr, 1, &prompt);
     if (rc) return rc;

@@ -544,22 +544,22 @@ __global__ __launch_bounds__(256) void paged_compact_kernel(PagedCacheView c, lo
 
 }  // namespace
 
-void launch_paged_plan(const PlanParams& p, hipStream_t s) {
+hipError_t launch_paged_plan(const PlanParams& p, hipStream_t s) {
     // a row per thread (256 chains of 166 k rows: 7.2 us; 2 rows 8.2, 4 rows 9.8, 8 rows 13.8), up to what runs side by side; one
     // workgroup per tree
     long wgs = (p.rows + kPlanThreads - 1) / kPlanThreads;
     wgs = wgs < 1 ? 1 : wgs > 512 ? 512 : wgs;
     if (p.parents && wgs < p.batch) wgs = p.batch;
-    paged_plan_kernel<<<(unsigned)wgs, kPlanThreads, 0, s>>>(p);
+    return launch(paged_plan_kernel, (unsigned)wgs, kPlanThreads, s, p);
 }
 
-void launch_paged_write(const PagedCacheView& c, int dim, int bf16, const void* k, const void* v, long k_row, long k_head, long v_row,
+hipError_t launch_paged_write(const PagedCacheView& c, int dim, int bf16, const void* k, const void* v, long k_row, long k_head, long v_row,
                         long v_head, const long* slots, long rows, hipStream_t s) {
     const long pairs = rows * c.heads, threads = pairs * (dim / 8);
-    if (!threads) return;
+    if (!threads) return hipSuccess;
     const unsigned grid = (unsigned)((threads + 255) / 256);
     const unsigned short *kk = static_cast<const unsigned short*>(k), *vv = static_cast<const unsigned short*>(v);
-#define MW_WRITE(BF, KV8, D) paged_write_kernel<BF, KV8, D><<<grid, 256, 0, s>>>(c, kk, vv, k_row, k_head, v_row, v_head, slots, pairs)
+#define MW_WRITE(BF, KV8, D) return launch(paged_write_kernel<BF, KV8, D>, grid, 256, s, c, kk, vv, k_row, k_head, v_row, v_head, slots, pairs)
     if (!c.ks) { if (dim == 64) MW_WRITE(false, false, 64); else MW_WRITE(false, false, 128); }       // 16-bit values are copied as they are
     else if (bf16) { if (dim == 64) MW_WRITE(true, true, 64); else MW_WRITE(true, true, 128); }
     else { if (dim == 64) MW_WRITE(false, true, 64); else MW_WRITE(false, true, 128); }
@@ -575,21 +575,23 @@ int accept_parts(long rows, int vocab) {
     return n < 1 ? 1 : n > kAcceptMaxParts ? kAcceptMaxParts : (int)n;
 }
 
-void launch_tree_accept(const AcceptParams& p, hipStream_t s) {
+hipError_t launch_tree_accept(const AcceptParams& p, hipStream_t s) {
     const int parts = accept_parts(p.rows, p.vocab);
     const int per = ((p.vocab + parts - 1) / parts + 7) / 8 * 8;
     float* pv = static_cast<float*>(p.workspace);
     int* pi = reinterpret_cast<int*>(pv + (long)p.rows * parts);
     if (p.rows > 0) {
         const unsigned grid = (unsigned)((long)p.rows * parts);
-        if (p.dtype == 0) accept_scan_kernel<float><<<grid, 256, 0, s>>>(static_cast<const float*>(p.logits), p.stride, p.vocab, p.suppress, parts, per, pv, pi);
-        else if (p.dtype == 1) accept_scan_kernel<f16><<<grid, 256, 0, s>>>(static_cast<const f16*>(p.logits), p.stride, p.vocab, p.suppress, parts, per, pv, pi);
-        else accept_scan_kernel<unsigned short><<<grid, 256, 0, s>>>(static_cast<const unsigned short*>(p.logits), p.stride, p.vocab, p.suppress, parts, per, pv, pi);
+        hipError_t e;
+        if (p.dtype == 0) e = launch(accept_scan_kernel<float>, grid, 256, s, static_cast<const float*>(p.logits), p.stride, p.vocab, p.suppress, parts, per, pv, pi);
+        else if (p.dtype == 1) e = launch(accept_scan_kernel<f16>, grid, 256, s, static_cast<const f16*>(p.logits), p.stride, p.vocab, p.suppress, parts, per, pv, pi);
+        else e = launch(accept_scan_kernel<unsigned short>, grid, 256, s, static_cast<const unsigned short*>(p.logits), p.stride, p.vocab, p.suppress, parts, per, pv, pi);
+        if (e != hipSuccess) return e;
     }
-    accept_walk_kernel<<<(unsigned)p.batch, 256, 0, s>>>(p, parts, pv, pi);
+    return launch(accept_walk_kernel, (unsigned)p.batch, 256, s, p, parts, pv, pi);
 }
 
-void launch_paged_compact(const PagedCacheView& c, int layers, long layer_stride, long scale_layer_stride, int dim, const int* table,
+hipError_t launch_paged_compact(const PagedCacheView& c, int layers, long layer_stride, long scale_layer_stride, int dim, const int* table,
                           long table_stride, int max_pages, const int* kept, const int* path, int path_cols, const int* count, int batch,
                           hipStream_t s) {
     const int esize = c.ks ? 1 : 2;
@@ -600,8 +602,8 @@ void launch_paged_compact(const PagedCacheView& c, int layers, long layer_stride
     // layers, 5 blocks: 7.3 us with 2 layers each, 8.6 with one.
     const long share = std::max(((long)blocks * batch * layers + 8191) / 8192, (long)(16 + path_cols - 1) / path_cols);
     const int groups = (int)((layers + share - 1) / share);
-    paged_compact_kernel<<<dim3(blocks, groups, batch), 256, 0, s>>>(c, layer_stride, scale_layer_stride, esize, dim, table, table_stride, max_pages,
-                                                                     kept, path, path_cols, count, layers);
+    return launch(paged_compact_kernel, dim3(blocks, groups, batch), 256, s, c, layer_stride, scale_layer_stride, esize, dim, table, table_stride, max_pages,
+                  kept, path, path_cols, count, layers);
 }
 
 }  // namespace mw

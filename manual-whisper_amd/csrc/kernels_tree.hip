@@ -675,7 +675,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeAttnParams p, int gr
 }
 
 template <typename T, bool KV8, int D>
-void launch_tree_t(const TreeAttnParams& p, hipStream_t s) {
+hipError_t launch_tree_t(const TreeAttnParams& p, hipStream_t s) {
     const int group = p.heads / p.c.heads;
     const long cols = (long)p.max_nodes * group;
     // 24 chains over 138 k tokens, 8 K/V heads of 128, narrow / wide: 16 columns 115 / 127 us bf16, 73 / 94 us e4m3; 24 columns, two
@@ -684,15 +684,15 @@ void launch_tree_t(const TreeAttnParams& p, hipStream_t s) {
     const int n_blocks = (int)((cols + block - 1) / block);
     const long pairs = ((long)p.n_units * p.c.heads + 7) / 8 * 8;
     const unsigned grid = (unsigned)(pairs * n_blocks);
-    if (block == 16) tree_attn_narrow_kernel<T, KV8, D><<<grid, 256, 0, s>>>(p, n_blocks, group);
-    else tree_attn_wide_kernel<T, KV8, D><<<grid, 256, 0, s>>>(p, n_blocks, group);
-    if (p.n_units > p.batch) {
+    const hipError_t e = launch(block == 16 ? tree_attn_narrow_kernel<T, KV8, D> : tree_attn_wide_kernel<T, KV8, D>, grid, 256, s, p, n_blocks, group);
+    if (e == hipSuccess && p.n_units > p.batch) {
         // few rows have few waves: a workgroup shares a row's units then (8 requests of 1 row, 32 heads, up to 80 units: 15.5 ->
         // 5.1 us); for many rows with a pair on every group of lanes it is faster without (32 trees, 8 units at most: 44 us shared)
         const long pairs = (long)p.batch * p.max_nodes * p.heads, groups = 256 / (D / 4);
-        if (pairs <= 4096) tree_join_kernel<T, D, true><<<(unsigned)pairs, 256, 0, s>>>(p, group);
-        else tree_join_kernel<T, D, false><<<(unsigned)((pairs + groups - 1) / groups), 256, 0, s>>>(p, group);
+        if (pairs <= 4096) return launch(tree_join_kernel<T, D, true>, (unsigned)pairs, 256, s, p, group);
+        return launch(tree_join_kernel<T, D, false>, (unsigned)((pairs + groups - 1) / groups), 256, s, p, group);
     }
+    return e;
 }
 
 }  // namespace
@@ -702,15 +702,15 @@ long tree_attn_workspace(int n_units, int batch, int kv_heads, int group, int ma
     return n_units > batch ? (long)n_units * kv_heads * max_nodes * group * (dim + 2) * 4 : 0;
 }
 
-void launch_tree_attention(const TreeAttnParams& p, hipStream_t s) {
-    if (!p.n_units || !p.batch || !p.max_nodes) return;
+hipError_t launch_tree_attention(const TreeAttnParams& p, hipStream_t s) {
+    if (!p.n_units || !p.batch || !p.max_nodes) return hipSuccess;
     const bool kv8 = p.c.ks != nullptr;
     if (p.dim == 64) {
-        if (p.bf16) { if (kv8) launch_tree_t<bf16, true, 64>(p, s); else launch_tree_t<bf16, false, 64>(p, s); }
-        else { if (kv8) launch_tree_t<f16, true, 64>(p, s); else launch_tree_t<f16, false, 64>(p, s); }
+        if (p.bf16) { if (kv8) return launch_tree_t<bf16, true, 64>(p, s); else return launch_tree_t<bf16, false, 64>(p, s); }
+        else { if (kv8) return launch_tree_t<f16, true, 64>(p, s); else return launch_tree_t<f16, false, 64>(p, s); }
     } else {
-        if (p.bf16) { if (kv8) launch_tree_t<bf16, true, 128>(p, s); else launch_tree_t<bf16, false, 128>(p, s); }
-        else { if (kv8) launch_tree_t<f16, true, 128>(p, s); else launch_tree_t<f16, false, 128>(p, s); }
+        if (p.bf16) { if (kv8) return launch_tree_t<bf16, true, 128>(p, s); else return launch_tree_t<bf16, false, 128>(p, s); }
+        else { if (kv8) return launch_tree_t<f16, true, 128>(p, s); else return launch_tree_t<f16, false, 128>(p, s); }
     }
 }
 

@@ -4,6 +4,9 @@
 #include <hip/hip_fp16.h>
 #include <stdint.h>
 
+#include <tuple>
+#include <type_traits>
+
 namespace mw {
 
 typedef _Float16 f16;
@@ -301,6 +304,17 @@ void launch_log_softmax_rows(float* z, int rows, int ld, int V, hipStream_t s);
 // out [rows][1 + J]: column 0 = z[r][blank], column 1 + j = z[r][tokens[j]], or for tokens[j] == -1 the largest z[r][v], v != blank
 void launch_ctc_gather(const float* z, int rows, int ld, int V, const int32_t* tokens, int J, int blank, float* out, hipStream_t s);
 
+// Queue a kernel and return this launch's own status: a launch by <<< >>> only leaves one behind (hipGetLastError), which may be an
+// earlier call's that its caller has not asked for yet.
+template <class... P, class... A>
+inline hipError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, hipStream_t s, A... a) {
+    std::tuple<std::remove_cv_t<P>...> values(static_cast<P>(a)...);
+    return std::apply([&](auto&... v) {
+        void* args[] = {const_cast<void*>(static_cast<const void*>(&v))...};
+        return hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, args, 0, s);
+    }, values);
+}
+
 // ---------------------------------------------------------------- drafted tokens over a K/V cache in pages
 // One layer of a cache in pages: row (page, head, offset) of K lies at k + page * page_stride + head * head_stride + offset *
 // token_stride elements (V likewise); 16-bit values, or e4m3 codes with one scale per row, ks / vs [page][head][1 << page_shift].
@@ -322,9 +336,9 @@ struct PlanParams {
     unsigned* mask; int mask_words;
     int* units; int* unit_start; int chunk_units, chunk_min;   // units null: none wanted
 };
-void launch_paged_plan(const PlanParams& p, hipStream_t s);
+hipError_t launch_paged_plan(const PlanParams& p, hipStream_t s);
 // k, v [rows][heads][dim] 16-bit (bf16: bfloat16, else fp16; a 16-bit cache holds the same type); strides in elements
-void launch_paged_write(const PagedCacheView& c, int dim, int bf16, const void* k, const void* v, long k_row, long k_head, long v_row,
+hipError_t launch_paged_write(const PagedCacheView& c, int dim, int bf16, const void* k, const void* v, long k_row, long k_head, long v_row,
                         long v_head, const long* slots, long rows, hipStream_t s);
 constexpr int kAcceptMaxNodes = 1024, kAcceptMaxParts = 64;
 struct AcceptParams {
@@ -336,8 +350,8 @@ struct AcceptParams {
     void* workspace;                                           // rows * accept_parts() * 8 bytes
 };
 int accept_parts(long rows, int vocab);
-void launch_tree_accept(const AcceptParams& p, hipStream_t s);
-void launch_paged_compact(const PagedCacheView& c, int layers, long layer_stride, long scale_layer_stride, int dim, const int* table,
+hipError_t launch_tree_accept(const AcceptParams& p, hipStream_t s);
+hipError_t launch_paged_compact(const PagedCacheView& c, int layers, long layer_stride, long scale_layer_stride, int dim, const int* table,
                           long table_stride, int max_pages, const int* kept, const int* path, int path_cols, const int* count, int batch,
                           hipStream_t s);
 struct TreeAttnParams {
@@ -373,6 +387,6 @@ void launch_draft_step(const DraftParams& p, int depth, int advance, hipStream_t
 void launch_draft_embed(const int* tokens, const int* positions, const f16* tok_emb, const f16* pos_emb, int D, int n_text_ctx, float* x, int rows,
                         hipStream_t s);
 long tree_attn_workspace(int n_units, int batch, int kv_heads, int group, int max_nodes, int dim);
-void launch_tree_attention(const TreeAttnParams& p, hipStream_t s);
+hipError_t launch_tree_attention(const TreeAttnParams& p, hipStream_t s);
 
 }  // namespace mw

@@ -35,6 +35,7 @@ struct OnDevice {
 };
 int launched(const char* who, hipError_t e) {
     if (e == hipSuccess) return MW_OK;
+    (void)hipGetLastError();                                 // told here, not by the next call that asks
     set_call_error(std::string(who) + ": " + hipGetErrorString(e));
     return MW_ERR_HIP;
 }
@@ -93,8 +94,7 @@ extern "C" int mw_paged_plan(const mw_plan_args* a, int device, void* stream) {
     static_assert(sizeof(long) == sizeof(int64_t), "");
     p.slots = reinterpret_cast<long*>(a->slots); p.mask = a->mask; p.mask_words = a->parents ? a->mask_words : 0;
     p.units = a->units; p.unit_start = a->unit_start; p.chunk_units = a->chunk_units; p.chunk_min = a->chunk_min;
-    launch_paged_plan(p, static_cast<hipStream_t>(stream));
-    return launched(who, hipGetLastError());
+    return launched(who, launch_paged_plan(p, static_cast<hipStream_t>(stream)));
 }
 
 extern "C" int mw_paged_write(const mw_paged_cache* cache, const void* k, const void* v, int dtype, int64_t k_row_stride, int64_t k_head_stride,
@@ -112,9 +112,8 @@ extern "C" int mw_paged_write(const mw_paged_cache* cache, const void* k, const 
     REFUSE_IF(rows * cache->n_heads * (cache->head_dim / 8) > kMaxThreads, "too many rows for one launch");
     OnDevice on(device);
     if (on.err != hipSuccess) return launched(who, on.err);
-    launch_paged_write(view_of(*cache), cache->head_dim, dtype == MW_BF16, k, v, k_row_stride, k_head_stride, v_row_stride, v_head_stride,
-                       reinterpret_cast<const long*>(slots), rows, static_cast<hipStream_t>(stream));
-    return launched(who, hipGetLastError());
+    return launched(who, launch_paged_write(view_of(*cache), cache->head_dim, dtype == MW_BF16, k, v, k_row_stride, k_head_stride, v_row_stride,
+                                            v_head_stride, reinterpret_cast<const long*>(slots), rows, static_cast<hipStream_t>(stream)));
 }
 
 static int check_attention(const char* who, const mw_tree_args* a) {
@@ -163,8 +162,7 @@ extern "C" int mw_tree_attention(const mw_tree_args* a, int device, void* stream
     p.out_row = a->out_row_stride; p.out_head = a->out_head_stride; p.table = a->table; p.table_stride = a->table_stride; p.max_pages = a->max_pages;
     p.kept = a->kept; p.row_start = a->row_start; p.units = a->units; p.unit_start = a->unit_start; p.n_units = a->n_units;
     p.mask = a->mask; p.mask_words = a->mask ? a->mask_words : 0; p.scale = a->scale; p.workspace = need ? static_cast<float*>(a->workspace) : nullptr;
-    launch_tree_attention(p, static_cast<hipStream_t>(stream));
-    return launched(who, hipGetLastError());
+    return launched(who, launch_tree_attention(p, static_cast<hipStream_t>(stream)));
 }
 
 static int check_accept(const char* who, const mw_accept_args* a) {
@@ -199,8 +197,7 @@ extern "C" int mw_tree_accept(const mw_accept_args* a, int device, void* stream)
     p.logits = a->logits; p.stride = a->logits_stride; p.dtype = a->dtype; p.rows = a->rows; p.vocab = a->vocab; p.batch = a->batch; p.depth = a->depth;
     p.suppress = a->suppress; p.tokens = a->tokens; p.parents = a->parents; p.row_start = a->row_start; p.best = a->best; p.path = a->path;
     p.count = a->count; p.out_tokens = a->out_tokens; p.workspace = a->workspace;
-    launch_tree_accept(p, static_cast<hipStream_t>(stream));
-    return launched(who, hipGetLastError());
+    return launched(who, launch_tree_accept(p, static_cast<hipStream_t>(stream)));
 }
 
 extern "C" int mw_paged_compact(const mw_paged_cache* cache, int32_t n_layers, int64_t layer_stride, const int32_t* table, int64_t table_stride,
@@ -219,7 +216,7 @@ extern "C" int mw_paged_compact(const mw_paged_cache* cache, int32_t n_layers, i
     REFUSE_IF(!table || !kept || !path || !count, "null array");
     OnDevice on(device);
     if (on.err != hipSuccess) return launched(who, on.err);
-    launch_paged_compact(view_of(*cache), n_layers, layer_stride, (int64_t)cache->n_pages * cache->n_heads * cache->page_size, cache->head_dim, table,
-                         table_stride, max_pages, kept, path, path_stride, count, batch, static_cast<hipStream_t>(stream));
-    return launched(who, hipGetLastError());
+    const int64_t scale_stride = (int64_t)cache->n_pages * cache->n_heads * cache->page_size;
+    return launched(who, launch_paged_compact(view_of(*cache), n_layers, layer_stride, scale_stride, cache->head_dim, table, table_stride, max_pages,
+                                              kept, path, path_stride, count, batch, static_cast<hipStream_t>(stream)));
 }

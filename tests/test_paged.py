@@ -961,3 +961,42 @@ def test_cut_requests_among_idle_ones_without_a_workspace(fresh):
         assert _lib.load().mw_tree_attention_workspace(C.byref(a)) == 0
         assert _lib.load().mw_tree_attention(C.byref(a), 0, torch.cuda.current_stream().cuda_stream) == 0
         assert torch.equal(out, got) and (guard == 7).all()
+
+
+def _hip():
+    """The HIP runtime that the library and torch run on."""
+    path = next(line.split()[-1] for line in open("/proc/self/maps") if "libamdhip64" in line)
+    return C.CDLL(path)
+
+
+@pytest.mark.gpu
+def test_an_error_that_somebody_else_left_is_not_the_calls():
+    """The runtime keeps a failed call's error until somebody asks: a call that follows neither fails for it nor takes it away."""
+    from manual_whisper_amd import paged
+    hip = _hip()
+    rng = np.random.default_rng(4)
+    cache, _, _ = _new_cache(rng, "f16", (4, 2, 16, 64))
+    rows = torch.randn(3, 2, 64, device="cuda", dtype=torch.float16)
+    slots = _dev([5, 17, 40], torch.int64)
+    table, kept, start = _dev([[0, 1, 2, 3]]), _dev([41]), _dev([0, 1])
+    units, first, one = _dev([[0, 0, 42, 1]]), _dev([0, 1]), _dev([1])
+    pool = paged.PagePool.create(4, 16, 1, 4)
+    logits, zero = torch.randn(1, 50, device="cuda"), _dev([0])
+    calls = [lambda: paged.write(cache, rows, rows, slots), lambda: pool.plan(kept, one, 1),
+             lambda: paged.tree_attention(rows[:1], cache, table, kept, start, units, first, 1),
+             lambda: paged.accept(logits, zero, zero, start, 1), lambda: paged.compact(cache, table, kept, _dev_path, one)]
+    _dev_path = _dev([[0]])
+    for call in calls:                                        # (torch's allocator has what the calls need)
+        call()
+    torch.cuda.synchronize()
+    for call in calls:
+        hip.hipGetLastError()
+        assert hip.hipSetDevice(4096) != 0                    # no such device
+        left = hip.hipPeekAtLastError()
+        try:
+            call()
+        finally:
+            still = hip.hipGetLastError()
+        assert still == left
+    torch.cuda.synchronize()
+    assert torch.equal(cache.k[1, :, 1], rows[1])
