@@ -14,7 +14,8 @@
 Thin wrappers over the C ABI (``mw_paged_*``, ``mw_tree_*`` in include/mwhip.h, where the semantics stand).  Tensors are
 device tensors of one GPU; the launches go to torch's current stream of that GPU and the calls return at once, so they order
 like torch's own operators and can be captured into a graph.  Outputs and workspaces come from torch's allocator; nothing
-is kept between calls.  There is no backward pass.  A bad argument raises ``EngineError``.
+is kept between calls.  There is no derivative, backward or forward: a tensor that requires a gradient is taken under
+``torch.no_grad()`` only, one with a tangent never.  A bad argument raises ``EngineError``.
 """
 from __future__ import annotations
 
@@ -24,6 +25,7 @@ import struct
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .engine import EngineError
@@ -111,12 +113,19 @@ def _table(t, device: int):
     return t.data_ptr(), batch, columns, stride if batch > 1 else columns        # (the stride of a dimension of one may be anything)
 
 
+def _no_gradient(t, name: str) -> None:
+    """Refuse a tensor that would have to pass a gradient on: there is no backward pass, and none forward either."""
+    if t.requires_grad and torch.is_grad_enabled():
+        _fail(f"{name} requires a gradient, and there is no backward pass (torch.no_grad() for its values)")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        _fail(f"{name} has a tangent, and there is no forward-mode derivative")
+
+
 def _rows3(t, name: str, device: int):
     """(address, row stride, head stride) of a [rows, heads, head_dim] tensor whose last dimension is dense."""
     if t.dim() != 3 or t.get_device() != device:
         _fail(f"{name} must be [rows, heads, head_dim] on cuda:{device}, got {tuple(t.shape)} on {t.device}")
-    if t.requires_grad:
-        _fail(f"{name} requires a gradient, and there is no backward pass")
+    _no_gradient(t, name)
     row, head, inner = t.stride()
     if inner != 1:
         _fail(f"{name} must have dense rows, got strides {t.stride()}")
@@ -318,8 +327,9 @@ def accept(logits, tokens, parents, row_start, depth: int, suppress=None):
     [batch], out_tokens [batch, depth]."""
     dev = _gpu_of(logits, "logits")
     dtype = _FLOATS.get(logits.dtype)
-    if logits.dim() != 2 or dtype is None or logits.requires_grad:
-        _fail(f"logits must be float [rows, vocab] without a gradient, got {logits.dtype} {tuple(logits.shape)}")
+    if logits.dim() != 2 or dtype is None:
+        _fail(f"logits must be float [rows, vocab], got {logits.dtype} {tuple(logits.shape)}")
+    _no_gradient(logits, "logits")
     rows, vocab = logits.shape
     stride, inner = logits.stride()
     if inner != 1 and vocab > 1:

@@ -1000,3 +1000,45 @@ def test_an_error_that_somebody_else_left_is_not_the_calls():
         assert still == left
     torch.cuda.synchronize()
     assert torch.equal(cache.k[1, :, 1], rows[1])
+
+
+def test_rows_that_require_gradients():
+    """Refused where a gradient would be lost, backward or forward, and taken as values under no_grad."""
+    from torch.autograd import forward_ad
+    from manual_whisper_amd import paged
+    from manual_whisper_amd.engine import EngineError
+    x = torch.zeros(2, 3, 64)
+    leaf = torch.zeros(2, 3, 64, requires_grad=True)
+    assert paged._rows3(x, "q", -1)[1:] == (192, 64)
+    for t in (leaf, leaf * 2):
+        with pytest.raises(EngineError, match="gradient"):
+            paged._rows3(t, "q", -1)
+        with torch.no_grad():
+            assert paged._rows3(t, "q", -1)[1:] == (192, 64)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        assert paged._rows3(x, "q", -1)[1:] == (192, 64)
+        for t in (dual, dual * 2):
+            with pytest.raises(EngineError, match="tangent"):
+                paged._rows3(t, "q", -1)
+            with torch.no_grad(), pytest.raises(EngineError, match="tangent"):       # no_grad leaves tangents as they are
+                paged._rows3(t, "q", -1)
+
+
+@pytest.mark.gpu
+def test_parameters_are_taken_under_no_grad():
+    from manual_whisper_amd import paged
+    from manual_whisper_amd.engine import EngineError
+    cache = paged.PagedCache.empty(1, 4, 2, 16, 64).layer(0)
+    rows = torch.randn(3, 2, 64, device="cuda", dtype=torch.float16)
+    leaf, slots = rows.clone().requires_grad_(), _dev([5, 17, 40], torch.int64)
+    args = (_dev([[0, 1, 2, 3]]), _dev([38]), _dev([0, 3]), _dev([[0, 0, 41, 1]]), _dev([0, 1]), 3)
+    calls = [lambda t: paged.write(cache, t, t, slots), lambda t: paged.tree_attention(t, cache, *args),
+             lambda t: paged.accept(t.view(3, 128), _dev([0] * 3), _dev([-1, 0, 1]), _dev([0, 3]), 3)]
+    for call in calls:
+        with pytest.raises(EngineError):
+            call(leaf)
+        with torch.no_grad():
+            got, want = call(leaf), call(rows)
+        assert got is None or all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(cache.k[2, :, 8], rows[2]) and torch.equal(cache.v[0, :, 5], rows[0])
