@@ -2,7 +2,7 @@
 // side?  A workgroup of 512 threads puts two waves on every SIMD; waves 0-3 run a chain-free loop of
 // v_mfma_f32_16x16x32_f16, waves 4-7 a loop of v_exp_f32 (or v_fma_f32).  One workgroup per CU, timed with events:
 // "both" close to the larger of the two alone = they overlap; close to the sum = they take turns.
-//   hipcc --offload-arch=gfx950 -O3 tools/coissue_probe.hip -o tools/coissue_probe
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/coissue_probe.hip -o tools/coissue_probe
 #include <hip/hip_runtime.h>
 #include <cstdio>
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));

@@ -1,6 +1,6 @@
 // Development aid: does an encoder product (MFMA-bound) overlap with the decode cross-attention of a decode group
 // (HBM-bound) when both are in flight on one GPU, or do the two take turns?
-//   hipcc -O3 -std=c++17 --offload-arch=gfx950 -I manual-whisper_amd/csrc tools/coreside_bench.hip \
+//   hipcc -O3 -std=c++17 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -I manual-whisper_amd/csrc tools/coreside_bench.hip \
 //         manual-whisper_amd/csrc/kernels_gemm.o manual-whisper_amd/csrc/kernels_dec.o -o tools/coreside_bench
 //   tools/coreside_bench [M N K [gemm_ms stream_ms [mode]]]
 // The product is launch_gemm (MW_GEMM_NO256=1 / MW_GEMM_CS=1 pick the other tile kernels), mode "", "gelu" or "resid";

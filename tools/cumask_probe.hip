@@ -1,5 +1,5 @@
 // Development aid: which compute-unit masks does hipExtStreamCreateWithCUMask accept on this device, and how
-// fast does a bandwidth-bound copy run on a stream limited to them?   hipcc --offload-arch=gfx950 -O2
+// fast does a bandwidth-bound copy run on a stream limited to them?   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

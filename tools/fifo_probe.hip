@@ -1,6 +1,6 @@
 // Development aid: what a kernel that reads L2-resident data (as a matrix product's tile loads do) and a kernel that
 // only issues MFMAs lose beside a saturating HBM read stream, and what the stream loses beside them.
-//   hipcc -O3 -std=c++17 --offload-arch=gfx950 tools/fifo_probe.hip -o tools/fifo_probe
+//   hipcc -O3 -std=c++17 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/fifo_probe.hip -o tools/fifo_probe
 // Three kernels, each timed alone and beside each of the others (two streams):
 //   stream : non-temporal read of 860 MB, 2240 workgroups x 256 threads, 16 loads of 16 bytes in flight per thread
 //   l2read : WG workgroups per CU x 256 threads re-reading a buffer of argv[2] MiB (default 2: resident in every XCD's

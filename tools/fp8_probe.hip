@@ -1,5 +1,5 @@
 // Developer harness: what the gfx950 fp8 conversion instructions do, against a software e4m3fn codec.
-//   hipcc -O3 --offload-arch=gfx950 tools/fp8_probe.hip -o tools/fp8_probe && tools/fp8_probe
+//   hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/fp8_probe.hip -o tools/fp8_probe && tools/fp8_probe
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdio.h>

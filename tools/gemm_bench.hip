@@ -1,5 +1,5 @@
 // Developer harness: checks launch_gemm against a naive GPU product on random fp16 data and times it.
-//   hipcc -O3 -std=c++17 --offload-arch=gfx950 -I manual-whisper_amd/csrc tools/gemm_bench.hip \
+//   hipcc -O3 -std=c++17 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -I manual-whisper_amd/csrc tools/gemm_bench.hip \
 //         manual-whisper_amd/csrc/kernels_gemm.o -o tools/gemm_bench
 //   tools/gemm_bench M N K [iters] [f8|gelu|qkv|resid]
 // "gelu", "qkv" (head split with transposed V, T = 1500) and "resid" (fp32 read-modify-write) time the encoder's other

@@ -5,7 +5,7 @@
 //                  per thread in flight (non-temporal), grid and D chosen on the command line
 //   probe kernel:  one wave, lane 0 chases pointers through a 1 GiB table of random links (every load misses the
 //                  caches), 4000 links, timed with the 100 MHz counter
-//   hipcc --offload-arch=gfx950 -O3 tools/lat_under_load.hip -o tools/lat_under_load
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/lat_under_load.hip -o tools/lat_under_load
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

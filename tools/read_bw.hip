@@ -1,7 +1,7 @@
 // Development aid: what does a read-only stream reach on this GPU?  Workgroups of 256 threads read disjoint contiguous
 // chunks (as the decode cross-attention does with its K/V ranges), U 16-byte loads per thread in flight, plain or
 // non-temporal; the sum goes to one float per workgroup so nothing is optimised away.
-//   hipcc --offload-arch=gfx950 -O3 tools/read_bw.hip -o tools/read_bw
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/read_bw.hip -o tools/read_bw
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

@@ -5,7 +5,7 @@
 //   mode 1: the same with both halves issued up front
 //   mode 2: workgroups that walk items (item, item + grid, ...) and issue the next item's halves as soon as the
 //           registers of the current one are consumed; the tail runs under those loads
-//   hipcc --offload-arch=gfx950 -O3 tools/read_bw2.hip -o tools/read_bw2
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/read_bw2.hip -o tools/read_bw2
 #include <hip/hip_runtime.h>
 #include <cstdio>
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
