@@ -180,3 +180,49 @@ def test_arguments_are_checked():
             eng.decode_drafted(n, drafts, nodes)
     eng.decode_drafted(2, good, 8)
     eng.close()
+
+
+# Polls of "all have ended" are four passes apart and one behind: up to eight passes more than the text needs.
+POLLS = 2 * 4
+
+
+def _passes(lens, nodes, max_new):
+    """Passes for texts that drafts have right: the prompt's, which yields a token, and one per `nodes` tokens."""
+    return 1 + max(-(-(min(n + 1, max_new) - 1) // nodes) for n in lens)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name,weights,kv,nodes,max_new", [("tiny", "fp8", "f16", 8, 48), ("tiny", "fp8", "fp8", 8, 48), ("micro", "f16", "f16", 64, 60),
+                                                           ("micro", "f16", "f16", 33, 60), ("micro", "f16", "f16", 17, 60)])
+def test_right_drafts_are_accepted(name, weights, kv, nodes, max_new):
+    """Drafts that are what drafted decoding itself returns take `nodes` tokens a pass, in fp8 engines and trees over two mask words too."""
+    n = 2
+    dims, w, pcm, eng = _engine(name, n * nodes, n, weights, kv)
+    eng.set_decode_options(synthetic_options(dims, max_new=max_new))
+    text, lens = eng.decode_drafted(n, [[] for _ in range(n)], nodes)
+    for _ in range(3):          # near-equal logits may fall differently in another grouping: what was decoded becomes the next draft
+        got, got_len = eng.decode_drafted(n, [[text[b, :lens[b]].tolist()] for b in range(n)], nodes)
+        same = (got == text).all()
+        text, lens = got, got_len
+        if same:
+            break
+    assert same and eng.stage_ms()["decode_steps"] <= _passes(lens, nodes, max_new) + POLLS < max_new
+    eng.close()
+
+
+@pytest.mark.gpu
+def test_right_drafts_are_accepted_up_to_the_end_of_text():
+    n, nodes, max_new = 3, 6, 60
+    dims, w, pcm, eng = _engine("micro", n * nodes, n)
+    base = synthetic_options(dims, max_new=max_new)
+    eng.set_decode_options(base)
+    ids, _, _ = eng.decode_greedy(n)
+    eng.set_decode_options(DecodeOptions(prompt=base.prompt, suppress=base.suppress, begin_suppress=base.begin_suppress, eot=int(ids[1, 20]),
+                                         max_new=max_new))
+    want, want_len, _ = eng.decode_greedy(n)
+    assert want_len[1] <= 20
+    eot = [int(ids[1, 20])]
+    got, got_len = eng.decode_drafted(n, [[want[b, :want_len[b]].tolist() + eot * int(want_len[b] < max_new)] for b in range(n)], nodes)
+    assert (got == want).all() and (got_len == want_len).all()
+    assert eng.stage_ms()["decode_steps"] <= _passes(want_len, nodes, max_new) + POLLS < max_new
+    eng.close()
