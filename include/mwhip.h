@@ -382,7 +382,7 @@ int mw_paged_write(const mw_paged_cache* cache, const void* k, const void* v, in
 typedef struct {
     mw_paged_cache cache;
     const void* q; int64_t q_row_stride, q_head_stride;         /* [rows][n_heads][head_dim] of `dtype`                   */
-    void* out; int64_t out_row_stride, out_head_stride;         /* likewise                                              */
+    void* out; int64_t out_row_stride, out_head_stride;         /* likewise; its rows share no memory (it may be q itself) */
     int32_t dtype;                        /* MW_F16 or MW_BF16; a 16-bit cache has the same type                        */
     int32_t n_heads;                      /* query heads: a multiple of the cache's; head h reads K/V head h / (n_heads / cache heads) */
     int32_t rows, batch;

@@ -6,6 +6,7 @@
 
 #include <math.h>
 #include <stdio.h>
+#include <stdlib.h>
 
 #include <string>
 
@@ -43,6 +44,13 @@ int launched(const char* who, hipError_t e) {
 constexpr int64_t kMaxThreads = (1LL << 32) - 256;           // of a launch along one dimension
 
 bool misaligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
+
+// whether rows of `dim` values, n x m of them at these strides, share memory
+bool overlapping(int64_t n, int64_t n_stride, int64_t m, int64_t m_stride, int64_t dim) {
+    const int64_t a = llabs(n_stride), b = llabs(m_stride);
+    if ((n > 1 && a < dim) || (m > 1 && b < dim)) return true;
+    return n > 1 && m > 1 && a < (m - 1) * b + dim && b < (n - 1) * a + dim;
+}
 
 int check_cache(const char* who, const mw_paged_cache* c) {
     REFUSE_IF(!c || !c->k || !c->v, "null cache");
@@ -147,6 +155,7 @@ extern "C" int mw_tree_attention(const mw_tree_args* a, int device, void* stream
     REFUSE_IF(!a->q || !a->out || !a->table || !a->kept || !a->row_start || !a->units || !a->unit_start, "null array");
     REFUSE_IF(misaligned(a->q, 16) || a->q_row_stride % 8 || a->q_head_stride % 8, "rows of q must start at multiples of 16 bytes");
     REFUSE_IF(misaligned(a->out, 8) || a->out_row_stride % 4 || a->out_head_stride % 4, "rows of out must start at multiples of 8 bytes");
+    REFUSE_IF(overlapping(a->rows, a->out_row_stride, a->n_heads, a->out_head_stride, a->cache.head_dim), "rows of out must not overlap");
     REFUSE_IF(misaligned(a->units, 16), "units must be 16-byte aligned");
     const int group = a->n_heads / a->cache.n_heads;
     const int64_t need = tree_attn_workspace(a->n_units, a->batch, a->cache.n_heads, group, a->max_nodes, a->cache.head_dim);

@@ -1042,3 +1042,30 @@ def test_parameters_are_taken_under_no_grad():
             got, want = call(leaf), call(rows)
         assert got is None or all(torch.equal(a, b) for a, b in zip(got, want))
     assert torch.equal(cache.k[2, :, 8], rows[2]) and torch.equal(cache.v[0, :, 5], rows[0])
+
+
+@pytest.mark.parametrize("rows,row,head,shared", [(8, 0, 64, True), (8, 1280, 0, True), (8, 64, 64, True), (8, 1216, 64, True), (8, 60, 8000, True),
+                                                  (8, 1280, 32, True), (8, 1280, -64, False), (8, 64, 512, False), (8, 64, 448, True), (1, 0, 64, False)])
+def test_rows_of_the_result_that_share_memory_are_refused(rows, row, head, shared):
+    """20 heads of 64: rows side by side, heads side by side, or neither (what passes this check meets the next one: units)."""
+    text = _refused(_lib.load().mw_tree_attention(C.byref(_tree_args(rows=rows, out_row_stride=row, out_head_stride=head, units=BAD + 8)), 0, None),
+                    "mw_tree_attention")
+    assert ("overlap" in text) == shared and ("units" in text) != shared
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fresh,target", [(3, 0), (3, 6), (40, 0), (40, 6)])
+def test_results_in_place_of_the_queries(fresh, target):
+    """`out` may be q itself (whole requests and cut ones), and not a tensor whose rows share memory."""
+    from manual_whisper_amd import paged
+    from manual_whisper_amd.engine import EngineError
+    rng = np.random.default_rng(fresh)
+    kept, n, page, heads, kv, dim = [300, 70], [fresh, 2], 16, 8, 2, 64
+    table, n_pages, start, see, words = _tree_case(rng, kept, n, page)
+    cache, _, _ = _new_cache(rng, "bf16", (n_pages, kv, page, dim))
+    q = torch.randn(start[-1], heads, dim, device="cuda").to(torch.bfloat16)
+    args = (cache, _dev(table), _dev(kept), _dev(start), *_units(kept, n, target, 64), fresh)
+    want = paged.tree_attention(q, *args, mask=_pack(see))
+    with pytest.raises(EngineError, match="overlap"):
+        paged.tree_attention(q, *args, mask=_pack(see), out=q[:1].clone().expand_as(q))
+    assert paged.tree_attention(q, *args, mask=_pack(see), out=q) is q and torch.equal(q, want)
