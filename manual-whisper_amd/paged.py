@@ -145,7 +145,7 @@ class PagedCache:
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         shape, strides, dtype = k.shape, k.stride(), k.dtype
-        if 1 in shape[-4:-2] and shape == v.shape:           # the stride of a dimension of one may be anything: the next one's, then
+        if 1 in shape[:-2] and shape == v.shape:           # the stride of a dimension of one may be anything: the next one's, then
             strides, other = _tight(shape, strides), _tight(shape, v.stride())
         else:
             other = v.stride()

@@ -1069,3 +1069,14 @@ def test_results_in_place_of_the_queries(fresh, target):
     with pytest.raises(EngineError, match="overlap"):
         paged.tree_attention(q, *args, mask=_pack(see), out=q[:1].clone().expand_as(q))
     assert paged.tree_attention(q, *args, mask=_pack(see), out=q) is q and torch.equal(q, want)
+
+
+def test_the_stride_between_layers_says_nothing_of_a_single_one():
+    """K and V of one layer out of caches of different depth: taken as far as the check of the device."""
+    from manual_whisper_amd import paged
+    from manual_whisper_amd.engine import EngineError
+    k, v = torch.zeros(1, 3, 2, 16, 64, dtype=torch.float16), torch.zeros(3, 2, 16, 64, dtype=torch.float16).as_strided((1, 3, 2, 16, 64), (8, 2048, 1024, 64, 1))
+    with pytest.raises(EngineError, match="on a GPU"):
+        paged.PagedCache(k, v)
+    with pytest.raises(EngineError, match="layout"):
+        paged.PagedCache(k, torch.zeros(1, 2, 3, 16, 64, dtype=torch.float16).transpose(1, 2))
