@@ -356,7 +356,9 @@ typedef struct {
     int32_t* units; int32_t* unit_start;  /* optional out: [batch + chunk_units][4] (request, first key, key behind the
                                            * last, units of that request; -1 behind the last unit) and [batch + 1]       */
     int32_t chunk_units;                  /* pieces wanted in all: requests are cut into equal pieces of multiples of 64
-                                           * keys, none shorter than chunk_min; 0: no request is cut                    */
+                                           * keys, none shorter than chunk_min; 0: no request is cut.  For long caches
+                                           * about 2048 over the K/V heads, and chunk_min at least 512 and 4 times the
+                                           * query columns of a K/V head                                                 */
     int32_t chunk_min;
 } mw_plan_args;
 
@@ -402,8 +404,11 @@ typedef struct {
  * zero, as are the rows of a request that was refused; rows behind the last request are left as they are.  Keys in a page
  * that does not exist (id outside 0..n_pages-1) count as not seen.  What a row does not see never reaches it, infinities
  * and NaN included.  Scores, maxima, sums and the result are held in fp32; weights are rounded once to `dtype` for the
- * product with V.  mw_tree_attention_workspace returns bytes (0: no workspace) or a negative mw_status; it reads neither
- * arrays nor workspace. */
+ * product with V (fp16: to half a step down to 2^-24 of a row's largest weight, below that to 2^-35 of it; e4m3: of the
+ * largest weight times the largest row scale of V that the row sees, to 2^-34).
+ * mw_tree_attention_workspace returns bytes (0: no workspace) or a negative mw_status; it reads neither arrays nor
+ * workspace.  The bytes grow with n_units * max_nodes: prompts are better given to a call of their own than mixed with
+ * requests of single rows. */
 int64_t mw_tree_attention_workspace(const mw_tree_args* args);
 int mw_tree_attention(const mw_tree_args* args, int device, void* stream);
 

@@ -5,6 +5,9 @@
 // All of them are bound by HBM or, at the sizes of one decode step, by the latency of a launch: each is one launch (accept:
 // two), nothing is allocated, nothing waits for the host, and every index that comes from device memory is checked
 // against its buffer before it is used.
+//
+// Times are medians of launches in a graph, three input sets in turn; "a where it is b" compares builds of one session by their
+// smallest times, which lie lower, by a third for the smallest launches.
 #include "mw_kernels.h"
 
 #include <algorithm>
@@ -19,7 +22,7 @@ namespace {
 // between workgroups.  A page popped from a stack entry that this very step pushes is looked up in the table of the request
 // that gives it back, so pops never wait for pushes.  Bound by latency: round trips to memory and the scans' barriers.  Sums go
 // through a wave by DPP and across waves once (with shuffles and a search per row: 13.4 us where it is 8.2).  16 trees of 8 nodes
-// 6.5 us (3 KB), 256 chains of 166 k rows in all 7.2 us (2 MB).
+// 8.0 us (3 KB), 256 chains of 166 k rows in all 7.9 us (2 MB).
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 constexpr int kPlanPer = kPlanMaxBatch / kPlanThreads;       // requests per thread of the prefix sums
 constexpr unsigned kFull = 1u << 30;                         // sums of counts stop here: above every capacity, and two of them fit 32 bits
@@ -268,8 +271,8 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanParams p) 
 // One thread moves 8 values of one (row, head): 16 bytes of K and of V in; the same bytes out, or 8 codes each.  HBM-bound:
 // every byte is touched once.  The row scale of an e4m3 cache needs the row's largest magnitude: a butterfly over the
 // D / 8 lanes that hold the row; a quotient is a product and one correction (divided out it is 30 us where it is now 26).
-// 128 rows of 20 heads of 64: 1.8 us, the launch.  19 k bf16 rows of 8 heads of 128 to e4m3: 25.7 us, 107 MB, of which 123 reach
-// memory (scales are 4 bytes here and there): 4.8 TB/s, a large copy's rate.
+// 128 rows of 20 heads of 64: 2.1 us, the launch.  19 k bf16 rows of 8 heads of 128 to e4m3: 26.2 us, 107 MB that become 123 at the
+// memory (scales are 4 bytes here and there): 4.7 TB/s, nearly a large copy's rate (4.9).
 template <bool BF> __device__ __forceinline__ void to_f32x8(uint4 u, float (&f)[8]) {
     const unsigned w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -344,8 +347,8 @@ __global__ __launch_bounds__(256) void paged_write_kernel(PagedCacheView c, cons
 // -------------------------------------------------------------------------------------------- accept
 // Arg-max of every row: HBM-bound, the logits once.  A row is cut into parts so that few rows still fill the chip; a thread
 // keeps its best (value, id) and looks at the suppressed ids only where a value would become its best.  Four loads of 16 bytes
-// ahead (eight: 9.2 us where it is 8.2, for parts of 4096 fp32).  1102 rows of 128000 bf16: 42.7 us, 282 MB, 6.6 TB/s; 128 rows of
-// 51866 fp32: 8.2 us, 27 MB, of which half is the first load's latency and the reduction's.
+// ahead (eight: 9.2 us where it is 8.2, for parts of 4096 fp32).  1102 rows of 128000 bf16: 44.7 us, 282 MB, 6.3 TB/s; 128 rows of
+// 51866 fp32: 10.2 us, 27 MB, of which half is the first load's latency and the reduction's.
 struct Best { float v; int i; };
 __device__ __forceinline__ Best better(Best a, Best b) {     // larger value, lower id on ties
     return b.v > a.v || (b.v == a.v && b.i < a.i) ? b : a;
@@ -411,7 +414,7 @@ __global__ __launch_bounds__(256) void accept_scan_kernel(const T* __restrict__ 
 }
 
 // The path of every tree: next[i] = the lowest child of i whose token is the arg-max of i's row, all nodes at once; then
-// one thread follows next[] from the root.  Bound by the latency of three dependent loads: 2.4 us for 16 trees of 8, 4.1 us for
+// one thread follows next[] from the root.  Bound by the latency of three dependent loads: 3.9 us for 16 trees of 8, 4.6 us for
 // 48 of up to 45.
 __global__ __launch_bounds__(256) void accept_walk_kernel(AcceptParams p, int parts, const float* __restrict__ part_v, const int* __restrict__ part_i) {
     __shared__ int next[kAcceptMaxNodes], ids[kAcceptMaxNodes];
@@ -456,7 +459,7 @@ __global__ __launch_bounds__(256) void accept_walk_kernel(AcceptParams p, int pa
 // of 4) and moves them for every accepted node: HBM-bound, 16 bytes in and out per piece.  A path ascends and path[i] >= i, so
 // what move i overwrites is only ever read by moves before it: a batch of moves is read as a whole, then written.  Pieces of 64
 // keep a workgroup's moves of 16 nodes in flight at once (256 pieces and node after node: 83 us where it is 51).  64 trees of up to
-// 60 nodes, 48 layers of 8 heads of 128 e4m3: 51 us, 213 MB in and out, 4.2 TB/s; 16 trees of 8, 32 layers of 20 heads of 64: 5.8 us, 14 MB.
+// 60 nodes, 48 layers of 8 heads of 128 e4m3: 52.7 us, 213 MB in and out, 4.0 TB/s; 16 trees of 8, 32 layers of 20 heads of 64: 6.5 us, 14 MB.
 constexpr int kCompactPieces = 64, kCompactPer = 4;
 template <typename V> __device__ __forceinline__ void move_pieces(char* const* column, int pieces, const long* src, const long* dst, int moves, long layer_off) {
     // item e = (move, piece), neighbours in a row side by side; kCompactPer items per thread are in flight

@@ -16,12 +16,13 @@
 // A request that is cut into several units leaves its partial results (fp32, with maximum and sum) in the workspace and a
 // second launch joins them.
 //
-// Measured (rows; K/V heads x head_dim; K/V read; this kernel, then the join):
-//   8 requests of 1 row, 207 k tokens of 8 x 128 bf16, 32 heads       849 MB   130 us (6.5 TB/s)                5.2 us
-//   16 trees of 8, 2.5 k tokens of 20 x 64 fp16, 20 heads              13 MB   8.9 us (latency: seven tiles)     no cut
-//   32 trees of 20..61, 80 k tokens of 8 x 128 bf16, 32 heads         329 MB   125 us (2.6 TB/s, 410 TFLOP/s)   14.1 us
-//   24 chains of 3..16, 138 k tokens of 8 x 128 e4m3, 64 heads        282 MB   109 us (2.6 TB/s, 313 TFLOP/s)   14.6 us
-// The wide trees' workgroups do not divide evenly over the CUs (30 % of the CU time is idle), 63 MB of partial results are written
+// Measured (rows; K/V heads x head_dim; K/V read; this kernel, then the join; medians of 498 launches in a graph, three input sets in
+// turn.  Further down "a where it is b" compares builds of one session by their smallest times, which lie up to 8 % lower):
+//   8 requests of 1 row, 207 k tokens of 8 x 128 bf16, 32 heads       849 MB           135 us (6.3 TB/s)                5.5 us
+//   16 trees of 8, 2.5 k tokens of 20 x 64 fp16, 20 heads              13 MB           9.7 us (latency: seven tiles)     no cut
+//   32 trees of 20..61, 80 k tokens of 8 x 128 bf16, 32 heads         329 MB, 51 GF   120 us (2.7 TB/s, 426 TFLOP/s)   14.5 us
+//   24 chains of 3..16, 138 k tokens of 8 x 128 e4m3, 64 heads        282 MB, 34 GF   105 us (2.7 TB/s, 326 TFLOP/s)   15.8 us
+// The wide trees' workgroups do not divide evenly over the CUs (24 % of the CU time is idle), 63 MB of partial results are written
 // and read, and 20 % of the products are padding.  Loads alone take 83 us, everything but the loads 80.
 #include "mw_kernels.h"
 
@@ -600,9 +601,9 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 3) void tree_attn_narrow_kernel(
     if (find_work(p, n_blocks, group, 16, w)) attend<T, KV8, D, 1, 4>(p, group, w, lds);
 }
 // Up to 128 columns a workgroup; how the four waves share columns and keys goes by the columns that this request has left: a wave
-// without columns would only stage.  (A wave of 64 columns reads half as much LDS per product but spills: 250 us; eight waves
-// of 256 columns read a request's rows once: 155 us, one workgroup per CU and its barriers; eight of 16 columns each 164 us;
-// queries in LDS and two tiles in flight 156 us.)
+// without columns would only stage.  (Both launches of the wide trees, where it was 142 us: a wave of 64 columns reads half as much
+// LDS per product but spills, 250; eight waves of 256 columns read a request's rows once, but one workgroup per CU waits at its
+// barriers, 155; eight of 16 columns each 164; queries in LDS and two tiles in flight 156.)
 template <typename T, bool KV8, int D>
 __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeAttnParams p, int n_blocks, int group) {
     __shared__ Shared<KV8, D> lds;
@@ -616,8 +617,8 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeAttnParams p
 
 // Rows of requests that were cut: the units' partial results, weighted by their maxima.  D / 4 lanes hold a (row, query head),
 // four head dims each.  SHARE: a workgroup per pair whose groups of lanes take the units in turn and are joined through LDS;
-// else every group has a pair of its own.  Bound by the bytes of the partial results (62 MB of wide trees in 14.2 us, 63 MB of
-// chains in 15.0: 4.3 TB/s); four loads ahead of a group that is alone with its pair (eight: 16.1 and 15.3 us), eight of one that shares.
+// else every group has a pair of its own.  Bound by the bytes of the partial results (63 MB of wide trees in 14.5 us, 67 MB of
+// chains in 15.8: 4.3 TB/s); four loads ahead of a group that is alone with its pair (eight: 16.1 and 15.3 us), eight of one that shares.
 template <typename T, int D, bool SHARE>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeAttnParams p, int group) {
     constexpr int LANES = D / 4, GROUPS = 256 / LANES, AHEAD = SHARE ? 8 : 4, STEP = SHARE ? GROUPS : 1;

@@ -2,7 +2,7 @@
 
     pool = PagePool.create(n_pages, page_size, batch, max_pages)       # tables and the stack of free pages
     cache = PagedCache.empty(layers, n_pages, heads, page_size, head_dim)
-    plan = pool.plan(kept, fresh, rows, parents)                       # pages, slots, positions, masks, work units
+    plan = pool.plan(kept, fresh, rows, parents, units=256)            # pages, slots, positions, masks, work units
     for i in range(layers):
         layer = cache.layer(i)
         write(layer, k, v, plan.slots)
@@ -238,8 +238,10 @@ class PagePool:
         """Plan a step in which request b appends ``fresh[b]`` rows behind its ``kept[b]`` tokens (``mw_paged_plan``).  ``rows``:
         capacity of the row arrays, at least the sum of ``fresh``.  ``parents`` int32 [rows]: trees of at most
         32 * ``mask_words`` nodes (default 8 words); None: chains.  ``units``: pieces that the attention's work is cut into
-        (0: requests are not cut), none shorter than ``chunk`` keys.  Tables and stack are updated in place; the plan takes
-        effect with ``commit``."""
+        (0: requests are not cut), none shorter than ``chunk`` keys.  Long caches need the cut, or few requests leave most of the
+        GPU idle: about 2048 pieces over the cache's heads (``max(16, 2048 // heads)``), ``chunk`` at least 512 and at least 4
+        times the query columns of a K/V head (rows of a request times query heads per K/V head); 0 where no request is
+        longer than some 512 keys.  Tables and stack are updated in place; the plan takes effect with ``commit``."""
         dev, batch = self.device, self.batch
         words = 0 if parents is None else 8 if mask_words is None else int(mask_words)
         if not (0 <= rows < 1 << 30 and 0 <= units <= 1 << 16 and 1 <= chunk < 1 << 31 and 0 <= words <= 8):
@@ -281,7 +283,9 @@ def tree_attention(q, cache: PagedCache, table, kept, row_start, units, unit_sta
                    out=None):
     """Attention of the step's rows over one cache layer (``mw_tree_attention``): ``q`` [rows, n_heads, head_dim] -> the same
     shape.  ``row_start``, ``units``, ``unit_start`` and (trees) ``mask`` are a plan's; ``max_nodes``: the most rows a request has.
-    ``scale`` defaults to 1 / sqrt(head_dim).  Rows behind the last request are left as they are in ``out`` (undefined without one)."""
+    ``scale`` defaults to 1 / sqrt(head_dim).  Where requests are cut, the workspace grows with the units times ``max_nodes``: prompts
+    are better attended to in a call of their own than among single rows.  Rows behind the last request are left as they are in
+    ``out`` (undefined without one)."""
     dev = cache._one().device
     pq, q_row, q_head = _rows3(q, "q", dev)
     rows, heads, dim = q.shape
