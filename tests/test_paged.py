@@ -1080,3 +1080,37 @@ def test_the_stride_between_layers_says_nothing_of_a_single_one():
         paged.PagedCache(k, v)
     with pytest.raises(EngineError, match="layout"):
         paged.PagedCache(k, torch.zeros(1, 2, 3, 16, 64, dtype=torch.float16).transpose(1, 2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,cache_kind", [("f16", "f16"), ("bf16", "bf16"), ("f16", "e4m3"), ("bf16", "e4m3")])
+@pytest.mark.parametrize("nodes,heads,target", [(6, 2, 0), (20, 4, 0), (40, 8, 0), (40, 8, 6)])
+def test_what_a_row_does_not_see_leaves_its_bits(nodes, heads, target, kind, cache_kind):
+    """K and V of a node of one branch, ordinary, large, infinite or NaN: the rows of the other branch keep their bits."""
+    from manual_whisper_amd import paged
+    rng = np.random.default_rng(nodes)
+    kept, n, page, kv, dim = [21, 300], [nodes, nodes], 16, 2, 64
+    table, n_pages, start, _, words = _tree_case(rng, kept, n, page)
+    see = np.zeros((start[-1], words * 32), bool)
+    for b in range(2):                                        # two branches under the root: odd nodes and even nodes
+        for i in range(nodes):
+            see[start[b] + i, 0] = True
+            see[start[b] + i, 2 - i % 2:i + 1:2] = True
+            see[start[b] + i, i] = True
+    cache, _, _ = _new_cache(rng, cache_kind, (n_pages, kv, page, dim))
+    q = torch.randn(start[-1], heads, dim, device="cuda").to(DT[kind])
+    args = (_dev(table), _dev(kept), _dev(start), *_units(kept, n, target, 64), nodes)
+    clean = paged.tree_attention(q, cache, *args, mask=_pack(see))
+    sees = torch.tensor(see[:, 3], device="cuda")
+    at = [(table[b][(kept[b] + 3) // page], (kept[b] + 3) % page) for b in range(2)]
+    e4m3 = cache_kind == "e4m3"
+    for value in (0x7E, 0x08, 0xFF) if e4m3 else (-3.0, 1000.0, 60000.0, float("inf"), float("nan")):
+        for scale in (1.0, 1e4, float("inf"), float("nan")) if e4m3 else (None,):
+            for pg, o in at:
+                cache.k[pg, :, o], cache.v[pg, :, o] = value, value
+                cache.k[pg, :, o, 1::2] = 0                   # scores of either sign and size
+                if e4m3:
+                    cache.k_scale[pg, :, o], cache.v_scale[pg, :, o] = scale, scale
+            got = paged.tree_attention(q, cache, *args, mask=_pack(see))
+            assert torch.equal(got[~sees], clean[~sees]), (value, scale)
+            assert not torch.equal(got[sees], clean[sees])
