@@ -1114,3 +1114,20 @@ def test_what_a_row_does_not_see_leaves_its_bits(nodes, heads, target, kind, cac
             got = paged.tree_attention(q, cache, *args, mask=_pack(see))
             assert torch.equal(got[~sees], clean[~sees]), (value, scale)
             assert not torch.equal(got[sees], clean[sees])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,cache_kind", [("f16", "f16"), ("bf16", "bf16"), ("f16", "e4m3")])
+@pytest.mark.parametrize("kept,fresh,target", [([0], [1100], 0), ([0], [1100], 9), ([0, 900, 40, 3], [700, 1, 9, 0], 0), ([513, 2500, 40, 3], [700, 1, 9, 1], 12)],
+                         ids=["prompt", "prompt cut", "mixed", "mixed cut"])
+def test_attention_of_prompts_and_of_mixed_batches(kept, fresh, target, kind, cache_kind):
+    """Chains of many hundred rows, alone and among single rows and short chains."""
+    from manual_whisper_amd import paged
+    rng = np.random.default_rng(len(kept) + target)
+    page, heads, kv, dim = 32, 4, 2, 64
+    table, n_pages, start, _, _ = _tree_case(rng, kept, fresh, page)
+    cache, k, v = _new_cache(rng, cache_kind, (n_pages, kv, page, dim))
+    q = torch.randn(start[-1], heads, dim, device="cuda").to(DT[kind])
+    got = paged.tree_attention(q, cache, _dev(table), _dev(kept), _dev(start), *_units(kept, fresh, target, 64), max(fresh))
+    want, size, big, vmax = ref.attention(q.double().cpu().numpy(), k, v, table, page, kept, start)
+    _close(got.double().cpu().numpy(), want, size, big, vmax, kind, dim, max(a + b for a, b in zip(kept, fresh)), cache_kind == "e4m3")
