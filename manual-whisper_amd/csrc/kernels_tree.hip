@@ -43,9 +43,9 @@ constexpr int KT = 64;                                       // keys of a tile
 
 // Weights are 2^(score - reference).  When a column's reference moves it goes kLow below the largest score, and it stays until a
 // score is more than kGap above it (positive: gap > 0 says that a column has seen a key).  fp16 holds full precision from 2^-14 to
-// 2^15, so its weights are kept high: the largest is 2^10 .. 2^14 (twice that beside an e4m3 row scale above 2^127), and one is
-// rounded by more than half a step of the type only where it is below 2^-24 of the largest, then by at most 2^-35 of it.  (With the
-// largest near 1 a long cache beside one dominant key loses its weights: 20 k tokens of e^-18 each came out as nothing.)
+// 2^15, so its weights are kept high: the largest is 2^10 .. 2^14, and one is rounded by more than half a step of the type only
+// where it is below 2^-24 of the largest, then by at most 2^-35 of it.  (With the largest near 1 a long cache beside one dominant
+// key loses its weights: 20 k tokens of e^-18 each came out as nothing.)
 template <typename T> struct Mat;
 template <> struct Mat<f16> {
     static __device__ __forceinline__ float4v mma32(short8v a, short8v b, float4v c) {
@@ -87,6 +87,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
     return r;
 }
+__device__ __forceinline__ int exponent(float x) { return (int)(__float_as_uint(x) >> 23 & 0xffu); }               // the field
 __device__ __forceinline__ float column_max(float v) {       // over the four lanes that share a query column
     v = fmaxf(v, __shfl_xor(v, 16));
     return fmaxf(v, __shfl_xor(v, 32));
@@ -250,10 +251,11 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
 #pragma unroll
     for (int qs = 0; qs < QT; ++qs) { ref[qs] = 0.f; gap[qs] = -INFINITY; l[qs] = 0.f; }
     // e4m3: weights are p_j times V's row scale relative to a power of two above every scale that the column has seen so far, so
-    // that they stay within fp16's range whatever the scales are; the accumulators are multiplied by it at the end
-    float vref[QT];
+    // that they stay within fp16's range whatever the scales are; the accumulators are multiplied by it at the end.  `vexp`: the
+    // largest exponent field of those scales, so that the power of two is 2^(vexp - 126)
+    int vexp[QT];
 #pragma unroll
-    for (int qs = 0; qs < QT; ++qs) vref[qs] = 0.f;
+    for (int qs = 0; qs < QT; ++qs) vexp[qs] = 0;
     // which of the 64 keys from node `first` on (negative: kept tokens before it) the row of node `n` sees
     auto visible = [&](int n, int first) -> unsigned long long {
         if (first <= -64) return ~0ull;
@@ -374,16 +376,16 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
                 for (int qs = 0; qs < QT; ++qs) big[qs] = all;
             }
 #pragma unroll
-            for (int qs = 0; qs < QT; ++qs) lift = lift || big[qs] > vref[qs];
+            for (int qs = 0; qs < QT; ++qs) lift = lift || exponent(big[qs]) > vexp[qs];
         }
         if (__any(lift)) {                                   // wave-uniform; a column moves for what it sees itself only
 #pragma unroll
             for (int qs = 0; qs < QT; ++qs) {
                 float f = 1.f;
-                if (KV8 && big[qs] > vref[qs]) {
-                    const float up = __uint_as_float(min((__float_as_uint(big[qs]) & 0x7f800000u) + 0x00800000u, 0x7f000000u));
-                    f = vref[qs] / up;
-                    vref[qs] = up;
+                if constexpr (KV8) {
+                    const int now = max(exponent(big[qs]), vexp[qs]);
+                    f = __builtin_ldexpf(1.f, vexp[qs] - now);
+                    vexp[qs] = now;
                 }
                 const float up = column_max(top[qs]);
                 const bool rises = up > gap[qs];
@@ -400,9 +402,6 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
                 for (int d = 0; d < ND; ++d) { o[d][qs][0] *= alpha * f; o[d][qs][1] *= alpha * f; o[d][qs][2] *= alpha * f; o[d][qs][3] *= alpha * f; }
             }
         }
-        float vinv[QT];                                      // (powers of two)
-#pragma unroll
-        for (int qs = 0; qs < QT; ++qs) vinv[qs] = KV8 && vref[qs] > 0.f ? 1.f / vref[qs] : 0.f;
         auto weigh = [&](auto some_unseen) {
             constexpr bool EDGE = decltype(some_unseen)::value;
 #pragma unroll
@@ -412,7 +411,7 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
                     vs4 = *reinterpret_cast<const float4v*>(&lds.scales[1][(wk * NK + i) * 16 + 4 * fg]);
                     if constexpr (!EDGE)                     // kept tokens only so far: the columns' references are the same
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) vs4[r] *= vinv[0];
+                        for (int r = 0; r < 4; ++r) vs4[r] = __builtin_ldexpf(vs4[r], 126 - vexp[0]);
                 }
 #pragma unroll
                 for (int qs = 0; qs < QT; ++qs)
@@ -422,7 +421,7 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
                         l[qs] += e;                          // of this lane's keys; the column's sum is formed at the end
                         if constexpr (!KV8) sc[i][qs][r] = e;
                         else if constexpr (!EDGE) sc[i][qs][r] = e * vs4[r];
-                        else sc[i][qs][r] = e == 0.f ? 0.f : e * (vs4[r] * vinv[qs]);          // whatever the scale of an unseen key
+                        else sc[i][qs][r] = e == 0.f ? 0.f : e * __builtin_ldexpf(vs4[r], 126 - vexp[qs]);        // whatever the scale of an unseen key
                     }
             }
         };
@@ -481,7 +480,9 @@ __device__ __forceinline__ void attend(const TreeAttnParams& p, int group, const
         l[qs] = column_sum(l[qs]);
         if constexpr (KV8)
 #pragma unroll
-            for (int d = 0; d < ND; ++d) { o[d][qs][0] *= vref[qs]; o[d][qs][1] *= vref[qs]; o[d][qs][2] *= vref[qs]; o[d][qs][3] *= vref[qs]; }
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[d][qs][r] = __builtin_ldexpf(o[d][qs][r], vexp[qs] - 126);
     }
     constexpr int DW = ND / WK;                              // 16-dim tiles of the result that a wave ends up with
     const int d0 = WK > 1 ? wk * DW : 0;
@@ -593,9 +594,10 @@ __device__ __forceinline__ bool find_work(const TreeAttnParams& p, int n_blocks,
     w.key1 = (int)min((long)min(u.z, p.max_pages << p.c.page_shift), (long)w.kept + last_node + 1);
     return true;
 }
-// At most 16 columns a workgroup: a stream of K/V through the compute units; registers are held down for more workgroups on each.
+// At most 16 columns a workgroup: a stream of K/V through the compute units; registers are held down for more workgroups on each
+// (8 requests of 1 row over 207 k tokens of 8 x 128 e4m3: 84 us with four, 87 with three).
 template <typename T, bool KV8, int D>
-__global__ __launch_bounds__(256, D == 64 ? 4 : 3) void tree_attn_narrow_kernel(TreeAttnParams p, int n_blocks, int group) {
+__global__ __launch_bounds__(256, D == 64 || KV8 ? 4 : 3) void tree_attn_narrow_kernel(TreeAttnParams p, int n_blocks, int group) {
     __shared__ Shared<KV8, D> lds;
     Work w;
     if (find_work(p, n_blocks, group, 16, w)) attend<T, KV8, D, 1, 4>(p, group, w, lds);
