@@ -347,8 +347,8 @@ __global__ __launch_bounds__(256) void paged_write_kernel(PagedCacheView c, cons
 // -------------------------------------------------------------------------------------------- accept
 // Arg-max of every row: HBM-bound, the logits once.  A row is cut into parts so that few rows still fill the chip; a thread
 // keeps its best (value, id) and looks at the suppressed ids only where a value would become its best.  Four loads of 16 bytes
-// ahead (eight: 9.2 us where it is 8.2, for parts of 4096 fp32).  1102 rows of 128000 bf16: 44.7 us, 282 MB, 6.3 TB/s; 128 rows of
-// 51866 fp32: 10.2 us, 27 MB, of which half is the first load's latency and the reduction's.
+// ahead (eight: 9.2 us where it is 8.2, for parts of 4096 fp32).  1102 rows of 128000 bf16: 44.6 us, 282 MB, 6.3 TB/s; 128 rows of
+// 51866 fp32: 10.3 us, 27 MB, of which half is the first load's latency and the reduction's.
 struct Best { float v; int i; };
 __device__ __forceinline__ Best better(Best a, Best b) {     // larger value, lower id on ties
     return b.v > a.v || (b.v == a.v && b.i < a.i) ? b : a;
@@ -459,7 +459,7 @@ __global__ __launch_bounds__(256) void accept_walk_kernel(AcceptParams p, int pa
 // of 4) and moves them for every accepted node: HBM-bound, 16 bytes in and out per piece.  A path ascends and path[i] >= i, so
 // what move i overwrites is only ever read by moves before it: a batch of moves is read as a whole, then written.  Pieces of 64
 // keep a workgroup's moves of 16 nodes in flight at once (256 pieces and node after node: 83 us where it is 51).  64 trees of up to
-// 60 nodes, 48 layers of 8 heads of 128 e4m3: 52.7 us, 213 MB in and out, 4.0 TB/s; 16 trees of 8, 32 layers of 20 heads of 64: 6.5 us, 14 MB.
+// 60 nodes, 48 layers of 8 heads of 128 e4m3: 52.6 us, 213 MB in and out, 4.0 TB/s; 16 trees of 8, 32 layers of 20 heads of 64: 6.5 us, 14 MB.
 constexpr int kCompactPieces = 64, kCompactPer = 4;
 template <typename V> __device__ __forceinline__ void move_pieces(char* const* column, int pieces, const long* src, const long* dst, int moves, long layer_off) {
     // item e = (move, piece), neighbours in a row side by side; kCompactPer items per thread are in flight

@@ -19,10 +19,10 @@
 // Measured (rows; K/V heads x head_dim; K/V read; this kernel, then the join; medians of 498 launches in a graph, three input sets in
 // turn.  Further down "a where it is b" compares builds of one session by their smallest times, which lie up to 8 % lower):
 //   8 requests of 1 row, 207 k tokens of 8 x 128 bf16, 32 heads       849 MB           135 us (6.3 TB/s)                5.5 us
-//   16 trees of 8, 2.5 k tokens of 20 x 64 fp16, 20 heads              13 MB           9.7 us (latency: seven tiles)     no cut
-//   32 trees of 20..61, 80 k tokens of 8 x 128 bf16, 32 heads         329 MB, 51 GF   120 us (2.7 TB/s, 426 TFLOP/s)   14.5 us
-//   24 chains of 3..16, 138 k tokens of 8 x 128 e4m3, 64 heads        282 MB, 34 GF   105 us (2.7 TB/s, 326 TFLOP/s)   15.8 us
-// The wide trees' workgroups do not divide evenly over the CUs (24 % of the CU time is idle), 63 MB of partial results are written
+//   16 trees of 8, 2.5 k tokens of 20 x 64 fp16, 20 heads              13 MB           9.8 us (latency: seven tiles)     no cut
+//   32 trees of 20..61, 80 k tokens of 8 x 128 bf16, 32 heads         329 MB, 51 GF   120 us (2.7 TB/s, 428 TFLOP/s)   14.5 us
+//   24 chains of 3..16, 138 k tokens of 8 x 128 e4m3, 64 heads        282 MB, 34 GF   104 us (2.7 TB/s, 328 TFLOP/s)   15.9 us
+// The wide trees' workgroups do not divide evenly over the CUs (23 % of the CU time is idle), 63 MB of partial results are written
 // and read, and 20 % of the products are padding.  Loads alone take 83 us, everything but the loads 80.
 #include "mw_kernels.h"
 
@@ -620,7 +620,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_wide_kernel(TreeAttnParams p
 // Rows of requests that were cut: the units' partial results, weighted by their maxima.  D / 4 lanes hold a (row, query head),
 // four head dims each.  SHARE: a workgroup per pair whose groups of lanes take the units in turn and are joined through LDS;
 // else every group has a pair of its own.  Bound by the bytes of the partial results (63 MB of wide trees in 14.5 us, 67 MB of
-// chains in 15.8: 4.3 TB/s); four loads ahead of a group that is alone with its pair (eight: 16.1 and 15.3 us), eight of one that shares.
+// chains in 15.9: 4.3 TB/s); four loads ahead of a group that is alone with its pair (eight: 16.1 and 15.3 us), eight of one that shares.
 template <typename T, int D, bool SHARE>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeAttnParams p, int group) {
     constexpr int LANES = D / 4, GROUPS = 256 / LANES, AHEAD = SHARE ? 8 : 4, STEP = SHARE ? GROUPS : 1;
